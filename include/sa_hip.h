@@ -78,7 +78,7 @@ typedef struct sa_paged_kv {
   int32_t query_heads;
   int32_t kv_heads;
   int32_t head_dim;
-  int32_t reserved;
+  int32_t reserved; /* SA_HIP_POOL_KV4: the pool holds 4-bit pages; otherwise unused */
 } sa_paged_kv;
 
 /* Budgeted selection parameters.
@@ -673,6 +673,129 @@ int sa_hip_decode_step_qkv(const sa_paged_kv* kv, const sa_qkv_producer* produce
                            const sa_select_params* params, float scale, int32_t* selected, int32_t* counts,
                            float* out, void* workspace, size_t workspace_bytes, int32_t splits, int32_t* status,
                            void* stream);
+
+/* ---- pages handed out and taken back on the GPU --------------------------- */
+/* No counterpart in the reference (its one sequence owns the whole store): a
+ * batch of requests shares one page pool, whose free pages are a stack,
+ * free_pages[0 .. *free_count), in device memory (room for num_pages
+ * entries).  Both calls work on any sa_paged_kv (the pool is not touched) and
+ * read nothing on the host, so they may be captured. */
+
+/* Room for new_tokens[b] more tokens of every sequence b (device, [batch],
+ * >= 0): pages for the blocks that kv->block_table does not hold yet are
+ * taken from the top of the stack, in the order of the sequences and of their
+ * blocks (page i taken is free_pages[*free_count - 1 - i]), and entered into
+ * kv->block_table.  Blocks [0, ceil(seq_len / 32)) are taken as held.
+ *   query_start     [batch + 1] int32: where each sequence's new tokens start
+ *                   in a ragged batch (exclusive sums of new_tokens).
+ *   slots           [max_tokens] int32: page * 32 + offset of each new token,
+ *                   in that order; -1 behind the last one.
+ *   positions       (optional) [max_tokens] int32: each new token's position
+ *                   in its sequence; -1 behind the last one.
+ *   seq_len_out     [batch]: seq_len + new_tokens; free_count_out: [1].  Either
+ *                   may be its input (in place); other overlaps are refused.
+ * Where the free pages, a table row or max_tokens do not suffice (status 8),
+ * or a length is negative or passes 32 bits (status 4), nothing is handed
+ * out: query_start is all 0, slots and positions are all -1, and the lengths
+ * and the count stay as they are.  A token whose page id is outside [0,
+ * num_pages) gets slot -1 and status 1.  A step that appends by itself
+ * (sa_hip_append_seal, sa_hip_decode_step) advances seq_len: pass another
+ * array as seq_len_out there.  num_pages < 2^26. */
+int sa_hip_reserve_tokens(const sa_paged_kv* kv, const int32_t* new_tokens, const int32_t* free_pages,
+                          const int32_t* free_count, int32_t max_tokens, int32_t* query_start, int32_t* slots,
+                          int32_t* positions, int32_t* seq_len_out, int32_t* free_count_out, int32_t* status,
+                          void* stream);
+/* The pages of every sequence b with finished[b] != 0 (device, [batch] int32)
+ * go back onto the stack, in the order of the sequences and of their blocks;
+ * seq_len_out[b] and kv->sealed[b] become 0 there, seq_len_out is seq_len
+ * elsewhere.  In place as above.  When the stack would grow past num_pages
+ * (status 8) or a length does not fit its table (status 4), nothing changes;
+ * a page id outside [0, num_pages) goes back as it is, with status 1. */
+int sa_hip_release_sequences(const sa_paged_kv* kv, const int32_t* finished, int32_t* free_pages,
+                             const int32_t* free_count, int32_t* seq_len_out, int32_t* free_count_out,
+                             int32_t* status, void* stream);
+
+/* ---- the KV cache in 4 bits ------------------------------------------------ */
+/* A second page format: sa_paged_kv with reserved = SA_HIP_POOL_KV4 and pool
+ * pointing to pages of sa_hip_kv4_page_bytes (5/16 of an FP16 page).  Tables,
+ * lengths, sealed blocks and representatives are as for FP16 pages, so the
+ * selection (sa_hip_score_select and its other forms) runs on it unchanged; entry points
+ * that read or write FP16 pages refuse it.  No counterpart in the reference.
+ * head_dim 64, 128 or 256; 1 to 16 query heads per KV head.
+ *
+ * A page is [kv_heads] records of 40 D bytes (D = head_dim, NG = D / 32,
+ * NC = D / 16).  Each row (a token's K or V of one head) has a scale and a
+ * minimum, both FP16, per 32 channels: value = scale * code + minimum.
+ * Token t = 16 T + 4 j + i (T < 2, j < 4, i < 4) has
+ *   key codes      byte t D/2 + (J NG + g) 4 + n/2, nibble n % 2: channel
+ *                  32 g + 8 J + n (J < 4, n < 8)
+ *   value codes    16 D + ((T 4 + j) 16 + r) 2 NC + i NC/2 + n/2, nibble
+ *                  n % 2: channel r NC + n (r < 16)
+ *   key scales     32 D + 2 (((T 4 + j) NG + g) 4 + i)
+ *   key minima     34 D + 2 (t NG + g)
+ *   value scales   36 D + 2 ((g 4 + j) 8 + 4 T + i)
+ *   value minima   38 D + 2 ((g 4 + j) 8 + 4 T + i)
+ * Quantising: values are limited to +-32000; minimum = fp16(min); scale =
+ * fp32((max - minimum) / 15), rounded up to 7 significant bits and to a
+ * multiple of 2^-24; code = round_half_even(fp32(fp32(x - minimum) / scale)) in
+ * [0, 15] (0 where the scale is 0).  A NaN makes its group's minimum NaN. */
+#define SA_HIP_POOL_KV4 0x4b563434
+
+/* Types of tokens, queries and outputs. */
+#define SA_HIP_F32 0
+#define SA_HIP_F16 1
+#define SA_HIP_BF16 2
+
+/* Bytes of a page (0 for a head_dim the format does not have). */
+size_t sa_hip_kv4_page_bytes(int32_t kv_heads, int32_t head_dim);
+
+/* Writes k and v of `tokens` tokens ([tokens][kv_heads][head_dim] of `type`,
+ * k_stride and v_stride elements between tokens) to their slots (device
+ * int32, page * 32 + offset, as sa_hip_reserve_tokens gives them; each slot
+ * once).  A negative slot is passed over, one past the pool too (status 1).
+ * k, v and their rows 16-byte aligned. */
+int sa_hip_kv4_store(const sa_paged_kv* kv, const void* k, const void* v, int32_t type, int64_t k_stride,
+                     int64_t v_stride, const int32_t* slots, int32_t tokens, int32_t* status, void* stream);
+/* Reads the values at `slots` back into k and v, rounded to `type`; rows of
+ * negative slots (and of slots past the pool, status 1) are left as they are. */
+int sa_hip_kv4_load(const sa_paged_kv* kv, void* k, void* v, int32_t type, int64_t k_stride, int64_t v_stride,
+                    const int32_t* slots, int32_t tokens, int32_t* status, void* stream);
+/* sa_hip_append_seal and sa_hip_seal on 4-bit pages: one token per sequence
+ * ([batch][kv_heads][head_dim] of `type`) at seq_len[b], then the seal; a
+ * representative is the mean of the block's keys as the cache holds them. */
+int sa_hip_kv4_append_seal(const sa_paged_kv* kv, const void* k, const void* v, int32_t type, int64_t k_stride,
+                           int64_t v_stride, int32_t local_tokens, int32_t* status, void* stream);
+int sa_hip_kv4_seal(const sa_paged_kv* kv, int32_t local_tokens, int32_t* status, void* stream);
+
+/* Workspace of the two attention calls below for up to `query_tokens` query
+ * rows (the batch, for one token a sequence).  It starts with arrival
+ * counters that the caller zeroes ONCE; every call leaves them at zero.  It
+ * serves every call of this cache's shape with at most that many rows and
+ * sequences.  Calls that share a workspace must not run concurrently. */
+size_t sa_hip_kv4_attention_workspace_bytes(const sa_paged_kv* kv, int32_t query_tokens);
+
+/* sa_hip_sparse_decode_attention on 4-bit pages: out[b][h] = softmax(scale *
+ * q[b][h] . K) V over the selected sealed blocks of h's group and the tail,
+ * or, with selected NULL (counts, select_groups and sel_stride unused), over
+ * every token of the sequence.  query ([batch][query_heads][head_dim], q_stride elements
+ * between tokens) and out (contiguous) of `type`; query 16-byte aligned in
+ * every row.  fp32 softmax and sums; fp32 queries enter the matrix cores as
+ * two FP16 parts.  A sequence without tokens gets zeros. */
+int sa_hip_kv4_decode_attention(const sa_paged_kv* kv, const void* query, int32_t type, int64_t q_stride,
+                                const int32_t* selected, const int32_t* counts, int32_t select_groups,
+                                int32_t sel_stride, float scale, void* out, void* workspace,
+                                size_t workspace_bytes, int32_t* status, void* stream);
+/* Causal attention of several tokens a sequence (a prompt's chunk, or
+ * drafted tokens) over its 4-bit pages, which hold them already: rows
+ * [query_start[b], query_start[b + 1]) of query (device int32 [batch + 1],
+ * ascending, at most query_tokens) are the last tokens of sequence b, and
+ * the row at position p sees the tokens [0, p].  Rows outside every
+ * sequence's range are left as they are.  A sequence with more rows than
+ * seq_len (status 4) gets zeros for those before its first token.  Starts
+ * that do not ascend within [0, query_tokens] attend nothing (status 4). */
+int sa_hip_kv4_prompt_attention(const sa_paged_kv* kv, const void* query, int32_t type, int64_t q_stride,
+                                const int32_t* query_start, int32_t query_tokens, float scale, void* out,
+                                void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 /* ---- synthetic data ------------------------------------------------------ */
 

@@ -42,9 +42,12 @@ hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // any_head_dim: the entry point also takes a head_dim other than 128 (any
-// multiple of 8 up to 512), which its general kernels serve.
-int check_geometry(const sa_paged_kv* kv, const char* op, bool any_head_dim = false) {
+// multiple of 8 up to 512), which its general kernels serve.  any_pool: it
+// does not touch the pool's pages, whatever their format.
+int check_geometry(const sa_paged_kv* kv, const char* op, bool any_head_dim = false, bool any_pool = false) {
   if (!kv) return fail(SA_HIP_EINVAL, "%s: null sa_paged_kv", op);
+  if (kv->reserved == SA_HIP_POOL_KV4 && !any_pool)
+    return fail(SA_HIP_EINVAL, "%s: the pool holds 4-bit pages (the sa_hip_kv4 entry points take them)", op);
   if (kv->head_dim != sa::kHeadDim) {
     if (!any_head_dim)
       return fail(SA_HIP_EINVAL, "%s: head_dim %d unsupported (this entry point is built for %d)", op,
@@ -436,8 +439,8 @@ static int online_check(const sa_paged_kv* kv, const sa_online_seal* seal, const
 
 static int select_launch(const sa_paged_kv* kv, const float* query, const sa_select_params* params,
                          int32_t* selected, int32_t* counts, float* scores, int32_t* status, const char* op,
-                         sa::SelectLaunch* l) {
-  if (int e = check_geometry(kv, op, true)) return e;
+                         sa::SelectLaunch* l, bool any_pool = false) {
+  if (int e = check_geometry(kv, op, true, any_pool)) return e;
   if (int e = check_reps(kv, op)) return e;
   if (!params || !query || !selected || !counts)
     return fail(SA_HIP_EINVAL, "%s: null params/query/selected/counts", op);
@@ -483,7 +486,7 @@ static int select_launch(const sa_paged_kv* kv, const float* query, const sa_sel
 int sa_hip_score_select(const sa_paged_kv* kv, const float* query, const sa_select_params* params,
                         int32_t* selected, int32_t* counts, float* scores, int32_t* status, void* stream) {
   sa::SelectLaunch l;
-  if (int e = select_launch(kv, query, params, selected, counts, scores, status, "score_select", &l)) return e;
+  if (int e = select_launch(kv, query, params, selected, counts, scores, status, "score_select", &l, true)) return e;
   if (sa::general_head_dim(l.head_dim)) {
     // the general scoring hands its scores to the selection launch
     if (!scores)
@@ -496,7 +499,7 @@ int sa_hip_score_select(const sa_paged_kv* kv, const float* query, const sa_sele
 int sa_hip_score_select_split(const sa_paged_kv* kv, const float* query, const sa_select_params* params,
                               int32_t* selected, int32_t* counts, float* scores, int32_t* status, void* stream) {
   sa::SelectLaunch l;
-  if (int e = select_launch(kv, query, params, selected, counts, scores, status, "score_select_split", &l)) return e;
+  if (int e = select_launch(kv, query, params, selected, counts, scores, status, "score_select_split", &l, true)) return e;
   if (!scores) return fail(SA_HIP_EINVAL, "score_select_split: the scores buffer is required");
   return check_hip(sa::launch_score_select_split(l, as_stream(stream)), "score_select_split launch");
 }
@@ -510,7 +513,7 @@ int sa_hip_score_select_chunked(const sa_paged_kv* kv, const float* query, const
                                 int32_t* selected, int32_t* counts, void* workspace, size_t workspace_bytes,
                                 int32_t* status, void* stream) {
   sa::SelectLaunch l;
-  if (int e = select_launch(kv, query, params, selected, counts, nullptr, status, "score_select_chunked", &l))
+  if (int e = select_launch(kv, query, params, selected, counts, nullptr, status, "score_select_chunked", &l, true))
     return e;
   if (sa::general_head_dim(l.head_dim))
     return fail(SA_HIP_EINVAL, "score_select_chunked: head_dim %d unsupported (128 only; sa_hip_score_select_split "
@@ -1385,6 +1388,297 @@ int sa_hip_stream_wait_event(void* stream, void* event) {
 }
 
 // ---- synthetic data --------------------------------------------------------------
+
+// ---- pages handed out and taken back ---------------------------------------------
+
+static int check_table(const sa_paged_kv* kv, const char* op) {
+  if (!kv) return fail(SA_HIP_EINVAL, "%s: null sa_paged_kv", op);
+  if (kv->batch <= 0 || kv->batch > 65535) return fail(SA_HIP_EINVAL, "%s: batch %d out of range", op, kv->batch);
+  if (kv->table_stride <= 0) return fail(SA_HIP_EINVAL, "%s: table_stride must be positive", op);
+  if (kv->num_pages <= 0 || kv->num_pages >= (1 << 26))
+    return fail(SA_HIP_EINVAL, "%s: num_pages must lie in [1, 2^26)", op);
+  if (!kv->block_table || !kv->seq_len) return fail(SA_HIP_EINVAL, "%s: null table/seq_len", op);
+  return SA_HIP_OK;
+}
+
+// 0: apart, 1: the same array, 2: anything between.
+static int overlap(const int32_t* a, const int32_t* b, int64_t n) {
+  if (a == b) return 1;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b), s = n * sizeof(int32_t);
+  return x < y + s && y < x + s ? 2 : 0;
+}
+
+static int check_in_place(const sa_paged_kv* kv, const int32_t* free_count, const int32_t* seq_len_out,
+                          const int32_t* free_count_out, const char* op, bool* in_place) {
+  const int lengths = overlap(kv->seq_len, seq_len_out, kv->batch);
+  const int counts = overlap(free_count, free_count_out, 1);
+  if (lengths == 2 || counts == 2)
+    return fail(SA_HIP_EINVAL, "%s: an output may be its input, but not overlap it otherwise", op);
+  *in_place = lengths || counts;
+  return SA_HIP_OK;
+}
+
+int sa_hip_reserve_tokens(const sa_paged_kv* kv, const int32_t* new_tokens, const int32_t* free_pages,
+                          const int32_t* free_count, int32_t max_tokens, int32_t* query_start, int32_t* slots,
+                          int32_t* positions, int32_t* seq_len_out, int32_t* free_count_out, int32_t* status,
+                          void* stream) {
+  const char* op = "reserve_tokens";
+  if (int e = check_table(kv, op)) return e;
+  if (!new_tokens || !free_pages || !free_count || !query_start || !seq_len_out || !free_count_out)
+    return fail(SA_HIP_EINVAL, "%s: null new_tokens/free_pages/free_count/query_start/seq_len_out/free_count_out", op);
+  if (max_tokens < 0 || (max_tokens > 0 && !slots)) return fail(SA_HIP_EINVAL, "%s: null slots", op);
+  sa::ReserveLaunch a{};
+  if (int e = check_in_place(kv, free_count, seq_len_out, free_count_out, op, &a.in_place)) return e;
+  a.table = kv->block_table;
+  a.seq_len = kv->seq_len;
+  a.new_tokens = new_tokens;
+  a.free_pages = free_pages;
+  a.free_count = free_count;
+  a.query_start = query_start;
+  a.slots = slots;
+  a.positions = positions;
+  a.seq_len_out = seq_len_out;
+  a.free_count_out = free_count_out;
+  a.status = status;
+  a.num_pages = kv->num_pages;
+  a.batch = kv->batch;
+  a.table_stride = kv->table_stride;
+  a.max_tokens = max_tokens;
+  return check_hip(sa::launch_reserve_tokens(a, as_stream(stream)), "reserve_tokens launch");
+}
+
+int sa_hip_release_sequences(const sa_paged_kv* kv, const int32_t* finished, int32_t* free_pages,
+                             const int32_t* free_count, int32_t* seq_len_out, int32_t* free_count_out,
+                             int32_t* status, void* stream) {
+  const char* op = "release_sequences";
+  if (int e = check_table(kv, op)) return e;
+  if (!finished || !free_pages || !free_count || !seq_len_out || !free_count_out || !kv->sealed)
+    return fail(SA_HIP_EINVAL, "%s: null finished/free_pages/free_count/seq_len_out/free_count_out/sealed", op);
+  sa::ReleaseLaunch a{};
+  if (int e = check_in_place(kv, free_count, seq_len_out, free_count_out, op, &a.in_place)) return e;
+  a.table = kv->block_table;
+  a.seq_len = kv->seq_len;
+  a.sealed = kv->sealed;
+  a.finished = finished;
+  a.free_pages = free_pages;
+  a.free_count = free_count;
+  a.seq_len_out = seq_len_out;
+  a.free_count_out = free_count_out;
+  a.status = status;
+  a.num_pages = kv->num_pages;
+  a.batch = kv->batch;
+  a.table_stride = kv->table_stride;
+  return check_hip(sa::launch_release_sequences(a, as_stream(stream)), "release_sequences launch");
+}
+
+// ---- the KV cache in 4 bits ---------------------------------------------------------
+
+static bool kv4_head_dim(int32_t d) { return d == 64 || d == 128 || d == 256; }
+
+static int check_kv4(const sa_paged_kv* kv, const char* op, bool tables) {
+  if (!kv) return fail(SA_HIP_EINVAL, "%s: null sa_paged_kv", op);
+  if (kv->reserved != SA_HIP_POOL_KV4)
+    return fail(SA_HIP_EINVAL, "%s: the pool does not hold 4-bit pages (reserved must be SA_HIP_POOL_KV4)", op);
+  if (!kv4_head_dim(kv->head_dim))
+    return fail(SA_HIP_EINVAL, "%s: head_dim %d unsupported (64, 128 or 256)", op, kv->head_dim);
+  if (kv->kv_heads <= 0 || kv->kv_heads > 65535 || kv->query_heads <= 0 || kv->query_heads % kv->kv_heads != 0)
+    return fail(SA_HIP_EINVAL, "%s: invalid GQA dimensions %d/%d", op, kv->query_heads, kv->kv_heads);
+  if (kv->query_heads / kv->kv_heads > sa::kKv4MaxGroup)
+    return fail(SA_HIP_EINVAL, "%s: %d query heads per KV head exceed %d", op, kv->query_heads / kv->kv_heads,
+                sa::kKv4MaxGroup);
+  if (kv->num_pages <= 0 || kv->num_pages >= (1 << 26))
+    return fail(SA_HIP_EINVAL, "%s: num_pages must lie in [1, 2^26)", op);
+  if (!kv->pool || !aligned16(kv->pool)) return fail(SA_HIP_EINVAL, "%s: null or unaligned pool (16 bytes)", op);
+  if (!tables) return SA_HIP_OK;
+  if (kv->batch <= 0 || kv->batch > 65535) return fail(SA_HIP_EINVAL, "%s: batch %d out of range", op, kv->batch);
+  if (kv->table_stride <= 0) return fail(SA_HIP_EINVAL, "%s: table_stride must be positive", op);
+  if (!kv->block_table || !kv->seq_len || !kv->sealed)
+    return fail(SA_HIP_EINVAL, "%s: null table/seq_len/sealed", op);
+  return SA_HIP_OK;
+}
+
+// Rows of [heads][head_dim] of `type`, `stride` elements apart.
+static int check_rows(const void* x, int32_t type, int64_t stride, int64_t heads, int32_t head_dim, const char* what,
+                      const char* op) {
+  if (type != SA_HIP_F32 && type != SA_HIP_F16 && type != SA_HIP_BF16)
+    return fail(SA_HIP_EINVAL, "%s: type %d unknown", op, type);
+  if (!x) return fail(SA_HIP_EINVAL, "%s: null %s", op, what);
+  const int64_t bytes = type == SA_HIP_F32 ? 4 : 2;
+  if (stride < heads * head_dim)
+    return fail(SA_HIP_EINVAL, "%s: %s rows of %lld elements are %lld apart", op, what,
+                static_cast<long long>(heads * head_dim), static_cast<long long>(stride));
+  if (!aligned16(x) || stride * bytes % 16 != 0)
+    return fail(SA_HIP_EINVAL, "%s: the rows of %s must be 16-byte aligned", op, what);
+  return SA_HIP_OK;
+}
+
+size_t sa_hip_kv4_page_bytes(int32_t kv_heads, int32_t head_dim) {
+  if (kv_heads <= 0 || !kv4_head_dim(head_dim)) return 0;
+  return static_cast<size_t>(kv_heads) * 40 * head_dim;
+}
+
+static int kv4_rows(const sa_paged_kv* kv, void* k, void* v, int32_t type, int64_t k_stride, int64_t v_stride,
+                    const int32_t* slots, int32_t tokens, int32_t* status, void* stream, bool load, const char* op) {
+  if (int e = check_kv4(kv, op, false)) return e;
+  if (tokens < 0) return fail(SA_HIP_EINVAL, "%s: %d tokens", op, tokens);
+  if (tokens == 0) return SA_HIP_OK;
+  if (int e = check_rows(k, type, k_stride, kv->kv_heads, kv->head_dim, "k", op)) return e;
+  if (int e = check_rows(v, type, v_stride, kv->kv_heads, kv->head_dim, "v", op)) return e;
+  if (!slots) return fail(SA_HIP_EINVAL, "%s: null slots", op);
+  if (static_cast<int64_t>(tokens) * kv->kv_heads > (1LL << 25))
+    return fail(SA_HIP_EINVAL, "%s: %d tokens x %d heads exceed 2^25 rows a call", op, tokens, kv->kv_heads);
+  sa::Kv4RowsLaunch a{};
+  a.pool = reinterpret_cast<uint8_t*>(kv->pool);
+  a.k = k;
+  a.v = v;
+  a.slots = slots;
+  a.status = status;
+  a.num_pages = kv->num_pages;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.tokens = tokens;
+  a.kv_heads = kv->kv_heads;
+  a.head_dim = kv->head_dim;
+  a.type = type;
+  a.load = load;
+  return check_hip(sa::launch_kv4_rows(a, as_stream(stream)), op);
+}
+
+int sa_hip_kv4_store(const sa_paged_kv* kv, const void* k, const void* v, int32_t type, int64_t k_stride,
+                     int64_t v_stride, const int32_t* slots, int32_t tokens, int32_t* status, void* stream) {
+  return kv4_rows(kv, const_cast<void*>(k), const_cast<void*>(v), type, k_stride, v_stride, slots, tokens, status,
+                  stream, false, "kv4_store");
+}
+
+int sa_hip_kv4_load(const sa_paged_kv* kv, void* k, void* v, int32_t type, int64_t k_stride, int64_t v_stride,
+                    const int32_t* slots, int32_t tokens, int32_t* status, void* stream) {
+  return kv4_rows(kv, k, v, type, k_stride, v_stride, slots, tokens, status, stream, true, "kv4_load");
+}
+
+static int kv4_seal_args(const sa_paged_kv* kv, int32_t local_tokens, int32_t* status, const char* op,
+                         sa::Kv4SealLaunch* a) {
+  if (int e = check_kv4(kv, op, true)) return e;
+  if (int e = check_reps(kv, op)) return e;
+  if (local_tokens < 0) return fail(SA_HIP_EINVAL, "%s: local_tokens must be >= 0", op);
+  a->pool = reinterpret_cast<uint8_t*>(kv->pool);
+  a->table = kv->block_table;
+  a->seq_len = kv->seq_len;
+  a->sealed = kv->sealed;
+  a->generation = kv->generation;
+  a->reps = kv->reps;
+  a->status = status;
+  a->num_pages = kv->num_pages;
+  a->batch = kv->batch;
+  a->table_stride = kv->table_stride;
+  a->kv_heads = kv->kv_heads;
+  a->rep_heads = kv->rep_heads;
+  a->rep_stride = kv->rep_stride;
+  a->local_tokens = local_tokens;
+  a->head_dim = kv->head_dim;
+  return SA_HIP_OK;
+}
+
+int sa_hip_kv4_append_seal(const sa_paged_kv* kv, const void* k, const void* v, int32_t type, int64_t k_stride,
+                           int64_t v_stride, int32_t local_tokens, int32_t* status, void* stream) {
+  const char* op = "kv4_append_seal";
+  sa::Kv4SealLaunch a{};
+  if (int e = kv4_seal_args(kv, local_tokens, status, op, &a)) return e;
+  if (int e = check_rows(k, type, k_stride, kv->kv_heads, kv->head_dim, "k", op)) return e;
+  if (int e = check_rows(v, type, v_stride, kv->kv_heads, kv->head_dim, "v", op)) return e;
+  a.k = k;
+  a.v = v;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.type = type;
+  return check_hip(sa::launch_kv4_append_seal(a, as_stream(stream)), op);
+}
+
+int sa_hip_kv4_seal(const sa_paged_kv* kv, int32_t local_tokens, int32_t* status, void* stream) {
+  sa::Kv4SealLaunch a{};
+  if (int e = kv4_seal_args(kv, local_tokens, status, "kv4_seal", &a)) return e;
+  return check_hip(sa::launch_kv4_seal(a, as_stream(stream)), "kv4_seal");
+}
+
+size_t sa_hip_kv4_attention_workspace_bytes(const sa_paged_kv* kv, int32_t query_tokens) {
+  if (!kv || query_tokens < 0 || kv->batch <= 0 || kv->kv_heads <= 0 || kv->query_heads < kv->kv_heads ||
+      !kv4_head_dim(kv->head_dim))
+    return 0;
+  return sa::kv4_attention_workspace_bytes(kv->batch, kv->query_heads, kv->kv_heads, kv->head_dim, query_tokens);
+}
+
+static int kv4_attention(const sa_paged_kv* kv, const void* query, int32_t type, int64_t q_stride, int32_t tokens,
+                         float scale, void* out, void* workspace, size_t workspace_bytes, int32_t* status,
+                         const char* op, sa::Kv4AttnLaunch* a) {
+  if (int e = check_rows(query, type, q_stride, kv->query_heads, kv->head_dim, "query", op)) return e;
+  if (!out || !aligned16(out)) return fail(SA_HIP_EINVAL, "%s: null or unaligned out (16 bytes)", op);
+  const uintptr_t bytes = type == SA_HIP_F32 ? 4 : 2, row = static_cast<uintptr_t>(kv->query_heads) * kv->head_dim;
+  const uintptr_t q0 = reinterpret_cast<uintptr_t>(query), o0 = reinterpret_cast<uintptr_t>(out);
+  const uintptr_t q1 = q0 + ((tokens - 1) * static_cast<uintptr_t>(q_stride) + row) * bytes, o1 = o0 + tokens * row * bytes;
+  if (q0 < o1 && o0 < q1 && !(q0 == o0 && q1 == o1))
+    return fail(SA_HIP_EINVAL, "%s: out may be the query's own buffer, but not overlap it otherwise", op);
+  const size_t need = sa_hip_kv4_attention_workspace_bytes(kv, tokens);
+  if (!workspace || workspace_bytes < need)
+    return fail(SA_HIP_EINVAL, "%s: workspace of %zu bytes needed, %zu given", op, need, workspace_bytes);
+  if (!aligned16(workspace)) return fail(SA_HIP_EINVAL, "%s: workspace must be 16-byte aligned", op);
+  if (static_cast<int64_t>(tokens) * kv->query_heads > (1LL << 30))
+    return fail(SA_HIP_EINVAL, "%s: %d tokens x %d heads exceed 2^30 rows a call", op, tokens, kv->query_heads);
+  a->pool = reinterpret_cast<const uint8_t*>(kv->pool);
+  a->table = kv->block_table;
+  a->seq_len = kv->seq_len;
+  a->sealed = kv->sealed;
+  a->query = query;
+  a->out = out;
+  a->workspace = workspace;
+  a->status = status;
+  a->num_pages = kv->num_pages;
+  a->q_stride = q_stride;
+  a->tokens = tokens;
+  a->batch = kv->batch;
+  a->table_stride = kv->table_stride;
+  a->query_heads = kv->query_heads;
+  a->kv_heads = kv->kv_heads;
+  a->head_dim = kv->head_dim;
+  a->type = type;
+  a->scale = scale;
+  return SA_HIP_OK;
+}
+
+int sa_hip_kv4_decode_attention(const sa_paged_kv* kv, const void* query, int32_t type, int64_t q_stride,
+                                const int32_t* selected, const int32_t* counts, int32_t select_groups,
+                                int32_t sel_stride, float scale, void* out, void* workspace,
+                                size_t workspace_bytes, int32_t* status, void* stream) {
+  const char* op = "kv4_decode_attention";
+  if (int e = check_kv4(kv, op, true)) return e;
+  if (selected) {
+    if (!counts) return fail(SA_HIP_EINVAL, "%s: null counts", op);
+    if (select_groups <= 0 || kv->kv_heads % select_groups != 0)
+      return fail(SA_HIP_EINVAL, "%s: select_groups must divide kv_heads", op);
+    if (sel_stride <= 0) return fail(SA_HIP_EINVAL, "%s: sel_stride must be positive", op);
+  }
+  sa::Kv4AttnLaunch a{};
+  if (int e = kv4_attention(kv, query, type, q_stride, kv->batch, scale, out, workspace, workspace_bytes, status, op, &a))
+    return e;
+  a.selected = selected;
+  a.counts = counts;
+  a.select_groups = select_groups;
+  a.sel_stride = sel_stride;
+  return check_hip(sa::launch_kv4_attention(a, as_stream(stream)), op);
+}
+
+int sa_hip_kv4_prompt_attention(const sa_paged_kv* kv, const void* query, int32_t type, int64_t q_stride,
+                                const int32_t* query_start, int32_t query_tokens, float scale, void* out,
+                                void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  const char* op = "kv4_prompt_attention";
+  if (int e = check_kv4(kv, op, true)) return e;
+  if (!query_start) return fail(SA_HIP_EINVAL, "%s: null query_start", op);
+  if (query_tokens < 0) return fail(SA_HIP_EINVAL, "%s: %d query_tokens", op, query_tokens);
+  if (query_tokens == 0) return SA_HIP_OK;
+  sa::Kv4AttnLaunch a{};
+  if (int e = kv4_attention(kv, query, type, q_stride, query_tokens, scale, out, workspace, workspace_bytes, status, op, &a))
+    return e;
+  a.query_start = query_start;
+  return check_hip(sa::launch_kv4_attention(a, as_stream(stream)), op);
+}
 
 int sa_hip_fill_synthetic_f16(uint16_t* dst, int64_t count, uint64_t seed, uint64_t first_index, void* stream) {
   if (!dst || count < 0) return fail(SA_HIP_EINVAL, "fill_synthetic_f16: bad arguments");

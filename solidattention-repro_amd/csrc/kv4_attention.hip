@@ -1,0 +1,978 @@
+// kv4_attention.hip — attention over the pages held in 4 bits, for one token
+// a sequence (every page, or selected blocks and the tail) and for several
+// (causal, ragged) (gfx950).
+//
+// out[r] = sum_t p_rt (s_t c_t + m_t) / sum_t p_rt, with p_rt = 2^(z_rt - max)
+// and z_rt = log2(e) scale q_r . (s_t c_t + m_t), per group of 32 channels.
+//
+// Everything runs on v_mfma_f32_16x16x32_f16, whose K is one group:
+//   scores   tile T: rows = tokens 16T.., columns = query rows.  The codes
+//            enter as 64 + c (the nibble moved into the mantissa of 64.0: one
+//            shift and one and-or for two), the accumulator starts at -64 sum
+//            q, and the group's sum takes its token's scale in fp32.  The
+//            minima are one more product: m_tg against the groups' sums of q.
+//   values   rows = channels, columns = query rows, products over tokens.
+//            The operand is c * s, exact in FP16 (7-bit scales); the minima
+//            and the denominator are one more product, with rows m_g and 1.
+// Both probabilities and maxima live where the score tile leaves them, lane
+// (query row, quarter of the tokens), which is the second product's operand.
+// fp32 queries and probabilities enter as a high and a low FP16 part (22
+// bits); 16-bit queries are exact in one part and the probabilities round to
+// FP16 (2^-11 relative).  Queries are scaled by a power of two per row, the
+// probabilities by 2^14: neither underflows in FP16 before 2^-38 of its largest.
+//
+// Work is split by pages, not by lists: the pages of all (sequence, KV head)
+// lists form one row of units, and each workgroup takes an equal share of it,
+// whatever the lists' lengths.  A list cut by a share's border is merged by the
+// last workgroup to finish it.
+#include "kv4_format.hpp"
+#include "sa_internal.hpp"
+
+#include <algorithm>
+
+namespace sa {
+namespace {
+
+using namespace kv4;
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kGroupsPerCu = 4;
+constexpr int kMaxGroups = 4096;   // workgroups, and arrival counters at the front of the workspace
+constexpr int kMinUnits = 8;       // pages a workgroup is worth starting for
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kProbShift = 14.0f;  // probabilities are held times 2^14
+
+struct Params {
+  const uint8_t* pool;
+  const int32_t* table;
+  const int32_t* seq_len;
+  const int32_t* sealed;
+  const int32_t* selected;
+  const int32_t* counts;
+  const int32_t* query_start;
+  const void* query;
+  void* out;
+  int32_t* status;
+  int32_t* arrive;
+  float* records;
+  int64_t* tile_info;  // prompt: [0] tiles, [1] units of one KV head
+  int64_t* tile_first; // units before a tile
+  int4* tiles;         // (sequence, first row, pages, -)
+  int64_t num_pages;
+  int64_t q_stride;
+  int32_t tokens;
+  int32_t batch;
+  int32_t table_stride;
+  int32_t sel_stride;
+  int32_t select_groups;
+  int32_t kv_per_sel;
+  int32_t query_heads;
+  int32_t kv_heads;
+  int32_t group;
+  int32_t type;
+  float qscale;
+};
+
+// ---- lists of pages -----------------------------------------------------------
+
+struct List {
+  const int32_t* sel;
+  int64_t len;   // tokens that may be read
+  int sealed;    // blocks the list's tail starts behind
+  int n_sel;
+  int total;     // pages
+};
+
+// One token a sequence: the selected blocks then the tail, or every page.
+// Inconsistent lengths are flagged and clamped to what can be read safely.
+__device__ inline List decode_list(const Params& p, int b, int sg) {
+  List L{nullptr, p.seq_len[b], 0, 0, 0};
+  bool bad = L.len < 0;
+  if (p.selected) {
+    L.sealed = p.sealed[b];
+    L.n_sel = p.counts[static_cast<int64_t>(b) * p.select_groups + sg];
+    L.sel = p.selected + (static_cast<int64_t>(b) * p.select_groups + sg) * p.sel_stride;
+    bad = bad || L.sealed < 0 || L.len < static_cast<int64_t>(L.sealed) * kPageTokens;
+    if (L.n_sel < 0 || L.n_sel > p.sel_stride) {
+      L.n_sel = 0;
+      flag_status(p.status, kStatusBadLength);
+    }
+  }
+  if (bad) {
+    flag_status(p.status, kStatusBadLength);
+    if (L.sealed < 0) L.sealed = 0;
+    L.len = static_cast<int64_t>(L.sealed) * kPageTokens;
+  }
+  const int64_t tail = L.len - static_cast<int64_t>(L.sealed) * kPageTokens;
+  L.total = L.n_sel + static_cast<int>((tail + kPageTokens - 1) / kPageTokens);
+  return L;
+}
+
+struct PageRef {
+  int32_t page;   // a readable page in any case
+  int32_t valid;  // its tokens (0: skip)
+};
+
+__device__ inline PageRef resolve(const Params& p, int b, const List& L, int i) {
+  PageRef r{0, 0};
+  if (i >= L.total) return r;
+  int64_t logical;
+  int valid = kPageTokens;
+  if (i < L.n_sel) {
+    logical = L.sel[i];
+    if (logical < 0 || logical >= L.sealed) {
+      flag_status(p.status, kStatusBadBlock);
+      return r;
+    }
+  } else {
+    logical = static_cast<int64_t>(L.sealed) + (i - L.n_sel);
+    const int64_t left = L.len - logical * kPageTokens;
+    if (left < kPageTokens) valid = static_cast<int>(left);
+  }
+  if (logical >= p.table_stride) {
+    flag_status(p.status, kStatusBadBlock);
+    return r;
+  }
+  const int32_t page = p.table[static_cast<int64_t>(b) * p.table_stride + logical];
+  if (page < 0 || page >= p.num_pages) {
+    flag_status(p.status, kStatusBadPage);
+    return r;
+  }
+  r.page = page;
+  r.valid = valid;
+  return r;
+}
+
+// ---- a record in a wave's registers ----------------------------------------------
+
+template <int D>
+struct Record {
+  using F = Format<D>;
+  uint32_t kc[2][F::NG];       // tile T: the lane's word of each group
+  uint32_t vc[2][F::NC / 2];   // tile T: 4 tokens x NC nibbles
+  uint32_t ks[2][F::NG * 2];   // tile T, group: scales of rows 4j..4j+3
+  uint32_t km[2][F::NG / 2];   // minima of token 16T + r
+  uint32_t vs[4];              // scales of the lane's channels, 8 slots
+  uint32_t vm[4];              // minima of group r % NG, 8 slots
+};
+
+template <int N>
+__device__ inline void load_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (N == 1) {
+    w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+  } else if constexpr (N == 2) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
+    w[0] = x.x, w[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 4 * i));
+      w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+    }
+  }
+}
+
+template <int D>
+__device__ inline void load_record(const uint8_t* rec, int lane, Record<D>& x) {
+  using F = Format<D>;
+  const int r = lane % 16, j = lane / 16;
+#pragma unroll
+  for (int T = 0; T < 2; ++T) {
+    load_words<F::NG>(rec + (16 * T + r) * (D / 2) + j * F::NG * 4, x.kc[T]);
+    load_words<F::NC / 2>(rec + F::kValueCodes + ((T * 4 + j) * 16 + r) * 2 * F::NC, x.vc[T]);
+    load_words<F::NG * 2>(rec + F::kKeyScales + (T * 4 + j) * F::NG * 8, x.ks[T]);
+    load_words<F::NG / 2>(rec + F::kKeyMins + (16 * T + r) * F::NG * 2, x.km[T]);
+  }
+  load_words<4>(rec + F::kValueScales + (r * F::NC / 32 * 4 + j) * 16, x.vs);
+  load_words<4>(rec + F::kValueMins + (r % F::NG * 4 + j) * 16, x.vm);
+}
+
+__device__ inline half8 as_half8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(half8, u32x4{a, b, c, d});
+}
+__device__ inline half2_t as_half2(uint32_t a) { return __builtin_bit_cast(half2_t, a); }
+__device__ inline uint32_t bits_of(half2_t a) { return __builtin_bit_cast(uint32_t, a); }
+
+// 8 nibbles as 64 + c, in the order (0,4), (1,5), (2,6), (3,7).
+__device__ inline half8 codes_plus64(uint32_t w) {
+  constexpr uint32_t kMask = 0x00F000F0u, kBase = 0x54005400u;  // 64.0: the mantissa's bits 4..7 count units
+  return as_half8(((w << 4) & kMask) | kBase, (w & kMask) | kBase, ((w >> 4) & kMask) | kBase,
+                  ((w >> 8) & kMask) | kBase);
+}
+
+// Nibble n (0..3) of both halves as FP16 integers times the pair of scales
+// (exact: 4 + 7 bits).
+template <int N>
+__device__ inline uint32_t scaled_codes(uint32_t y, uint32_t scales) {
+  half2_t c;
+  const uint32_t w = N < 2 ? y : y >> 8;
+  if constexpr (N % 2 == 0)
+    c = as_half2((w & 0x000F000Fu) | 0x64006400u) - half2_t{1024, 1024};
+  else
+    c = as_half2((w & 0x00F000F0u) | 0x54005400u) - half2_t{64, 64};
+  return bits_of(c * as_half2(scales));
+}
+
+__device__ inline f32x4 mfma(half8 a, half8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// The value operand of channel n of every row: slots 8j.. of tiles 0 and 1.
+template <int D, int N>
+__device__ inline half8 value_operand(const Record<D>& x) {
+  uint32_t w[4];
+#pragma unroll
+  for (int T = 0; T < 2; ++T) {
+    uint32_t p01, p23;
+    if constexpr (D == 64) {  // 16 bits a token: neighbours share a word
+      p01 = x.vc[T][0];
+      p23 = x.vc[T][1];
+    } else {
+      constexpr int kStep = D / 128;  // words a token
+      constexpr int kWord = N / 8;
+      constexpr uint32_t kSel = N % 8 < 4 ? 0x05040100u : 0x07060302u;
+      p01 = __builtin_amdgcn_perm(x.vc[T][kStep + kWord], x.vc[T][kWord], kSel);
+      p23 = __builtin_amdgcn_perm(x.vc[T][3 * kStep + kWord], x.vc[T][2 * kStep + kWord], kSel);
+    }
+    w[2 * T] = scaled_codes<N % 4>(p01, x.vs[2 * T]);
+    w[2 * T + 1] = scaled_codes<N % 4>(p23, x.vs[2 * T + 1]);
+  }
+  return as_half8(w[0], w[1], w[2], w[3]);
+}
+
+// ---- the query rows and the state of a wave -------------------------------------
+
+// Row r of tile rt of the list's rows: the lane's operand of the scores, the
+// sums of q, and the row's factor from products to exponents of 2.
+template <int D, int RT, bool kFine>
+struct Rows {
+  using F = Format<D>;
+  half8 hi[RT][F::NG];
+  half8 lo[RT][kFine ? F::NG : 1];
+  float base[RT][F::NG];  // -64 sum q of a group
+  half8 sums[RT];         // operand of the minima
+  float factor[RT];
+  int64_t limit[RT];      // last position the row sees
+};
+
+__device__ inline float ldexp2(float x, int e) { return __builtin_ldexpf(x, e); }
+
+template <int D, int RT, bool kFine>
+__device__ inline void load_rows(const Params& p, Rows<D, RT, kFine>& q, int64_t token0, int n_tokens, int head0,
+                                 int row0, int64_t limit0, int lane) {
+  using F = Format<D>;
+  const int r = lane % 16, j = lane / 16;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int row = row0 + rt * 16 + r;
+    const int token = row / p.group;
+    const bool live = token < n_tokens;
+    q.limit[rt] = live ? limit0 + token : limit0 + (n_tokens - 1);
+    float x[F::NG][8];
+    float top = 0.0f;
+#pragma unroll
+    for (int g = 0; g < F::NG; ++g) {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) x[g][n] = 0.0f;
+      if (live)
+        load8(p.query, (token0 + token) * p.q_stride + static_cast<int64_t>(head0 + row % p.group) * D + 32 * g + 8 * j,
+              p.type, x[g]);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) top = fmaxf(top, fabsf(x[g][n]));
+    }
+    top = xor_max<32>(xor_max<16>(top));
+    // the row's largest value into [1, 2): a power of two, exact
+    const int e = top > 0.0f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+    q.factor[rt] = ldexp2(p.qscale, e);
+    float sum[F::NG];
+#pragma unroll
+    for (int g = 0; g < F::NG; ++g) {
+      half8 hi, lo;
+      float s = 0.0f;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const int c = n / 2 + (n % 2) * 4;  // operand order (0,4), (1,5), ...
+        const float v = ldexp2(x[g][c], -e);
+        hi[n] = static_cast<_Float16>(v);
+        lo[n] = static_cast<_Float16>(v - static_cast<float>(hi[n]));
+        s += static_cast<float>(hi[n]);
+        if constexpr (kFine) s += static_cast<float>(lo[n]);
+      }
+      q.hi[rt][g] = hi;
+      if constexpr (kFine) q.lo[rt][g] = lo;
+      s = xor_sum<32>(xor_sum<16>(s));
+      q.base[rt][g] = -64.0f * s;
+      sum[g] = s;
+    }
+    // products of the minima: NG slots of high parts, NG of low ones
+    half8 op{};
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      float v = 0.0f;
+      bool low = false;
+      if constexpr (F::NG == 8) {
+        v = j < 2 ? sum[n] : 0.0f;
+        low = j == 1;
+      } else if (n < 2 * F::NG) {
+        v = j == 0 ? sum[n % F::NG] : 0.0f;
+        low = n >= F::NG;
+      }
+      const _Float16 h = static_cast<_Float16>(v);
+      op[n] = low ? static_cast<_Float16>(v - static_cast<float>(h)) : h;
+    }
+    q.sums[rt] = op;
+  }
+}
+
+template <int D, int RT>
+struct State {
+  using F = Format<D>;
+  float m[RT];
+  f32x4 acc[RT][F::NC];  // channel (4j + i) NC + n of query row r
+  f32x4 tail[RT];        // rows 0..NG-1: minima of each group; row NG: the denominator
+  __device__ inline void reset() {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m[rt] = kNegInf;
+      tail[rt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int n = 0; n < F::NC; ++n) acc[rt][n] = f32x4{0, 0, 0, 0};
+    }
+  }
+};
+
+// Masks the pair of slots (2q, 2q + 1) of the lane beyond `valid` tokens.
+__device__ inline uint32_t slot_mask(int q, int j, int valid) {
+  const int t = 16 * (q / 2) + 4 * j + 2 * (q % 2);
+  return (t < valid ? 0x0000FFFFu : 0u) | (t + 1 < valid ? 0xFFFF0000u : 0u);
+}
+
+template <int D, int RT, int N>
+__device__ inline void add_values(const Record<D>& x, const half8 (&ph)[RT], const half8 (&pl)[RT], bool fine,
+                                  State<D, RT>& st) {
+  const half8 v = value_operand<D, N>(x);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    st.acc[rt][N] = mfma(v, ph[rt], st.acc[rt][N]);
+    if (fine) st.acc[rt][N] = mfma(v, pl[rt], st.acc[rt][N]);
+  }
+  if constexpr (N + 1 < Format<D>::NC) add_values<D, RT, N + 1>(x, ph, pl, fine, st);
+}
+
+// Attends one page: `valid` tokens, the first at position pos; kCausal: a
+// row sees the tokens up to its limit.
+template <int D, int RT, bool kFine, bool kCausal>
+__device__ inline void attend(Record<D>& x, int valid, int64_t pos, int64_t first_limit, const Rows<D, RT, kFine>& q,
+                              State<D, RT>& st, int lane) {
+  using F = Format<D>;
+  const int r = lane % 16, j = lane / 16;
+  const bool cut = kCausal && pos + kPageTokens - 1 > first_limit;  // some row does not see all of it
+
+  f32x4 z[RT][2];
+#pragma unroll
+  for (int T = 0; T < 2; ++T) {
+    half8 mins;
+    {
+      const bool on = F::NG == 8 ? j < 2 : j == 0;
+      uint32_t w[F::NG / 2];
+#pragma unroll
+      for (int i = 0; i < F::NG / 2; ++i) w[i] = on ? x.km[T][i] : 0u;
+      if constexpr (F::NG == 8)
+        mins = as_half8(w[0], w[1], w[2], w[3]);
+      else if constexpr (F::NG == 4)
+        mins = as_half8(w[0], w[1], w[0], w[1]);
+      else
+        mins = as_half8(w[0], w[0], 0u, 0u);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) z[rt][T] = mfma(mins, q.sums[rt], f32x4{0, 0, 0, 0});
+#pragma unroll
+    for (int g = 0; g < F::NG; ++g) {
+      const half8 k = codes_plus64(x.kc[T][g]);
+      const uint32_t s01 = x.ks[T][2 * g], s23 = x.ks[T][2 * g + 1];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float b = q.base[rt][g];
+        f32x4 d = mfma(k, q.hi[rt][g], f32x4{b, b, b, b});
+        if constexpr (kFine) d = mfma(k, q.lo[rt][g], d);
+        z[rt][T][0] = __builtin_fmaf(lo_h2f(s01), d[0], z[rt][T][0]);
+        z[rt][T][1] = __builtin_fmaf(hi_h2f(s01), d[1], z[rt][T][1]);
+        z[rt][T][2] = __builtin_fmaf(lo_h2f(s23), d[2], z[rt][T][2]);
+        z[rt][T][3] = __builtin_fmaf(hi_h2f(s23), d[3], z[rt][T][3]);
+      }
+    }
+  }
+
+  half8 ph[RT], pl[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    float e[8];
+#pragma unroll
+    for (int n = 0; n < 8; ++n) e[n] = z[rt][n / 4][n % 4] * q.factor[rt];
+    if (valid < kPageTokens || cut) {
+      int seen = valid;
+      if (kCausal) {
+        const int64_t left = q.limit[rt] - pos + 1;
+        if (left < seen) seen = left < 0 ? 0 : static_cast<int>(left);
+      }
+#pragma unroll
+      for (int n = 0; n < 8; ++n) e[n] = 16 * (n / 4) + 4 * j + n % 4 < seen ? e[n] : kNegInf;
+    }
+    float top = e[0];
+#pragma unroll
+    for (int n = 1; n < 8; ++n) top = fmaxf(top, e[n]);
+    top = xor_max<32>(xor_max<16>(top));
+    if (__any(top > st.m[rt])) {
+      const bool up = top > st.m[rt];
+      const float f = up ? __builtin_amdgcn_exp2f(st.m[rt] - top) : 1.0f;
+      st.m[rt] = up ? top : st.m[rt];
+      st.tail[rt] *= f;
+#pragma unroll
+      for (int n = 0; n < F::NC; ++n) st.acc[rt][n] *= f;
+    }
+    const float off = (st.m[rt] == kNegInf ? 0.0f : st.m[rt]) - kProbShift;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const float v = __builtin_amdgcn_exp2f(e[n] - off);
+      ph[rt][n] = static_cast<_Float16>(v);
+      if constexpr (kFine) pl[rt][n] = static_cast<_Float16>(v - static_cast<float>(ph[rt][n]));
+    }
+  }
+
+  // rows of the last product: the groups' minima, then ones
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (valid < kPageTokens) {
+      const uint32_t mask = slot_mask(i, j, valid);  // what lies there is not the sequence's, and may be NaN
+      x.vs[i] &= mask;
+      x.vm[i] &= mask;
+    }
+    w[i] = r < F::NG ? x.vm[i] : r == F::NG ? 0x3C003C00u : 0u;
+  }
+  // A NaN minimum in a page that only some rows see wholly: 0 * NaN would
+  // reach the others, so it is taken out and added to the rows that see it.
+  if constexpr (kCausal) {
+    if (cut) {
+      uint64_t nan[8];
+      bool any = false;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const uint16_t h = static_cast<uint16_t>(w[n / 2] >> (16 * (n % 2)));
+        nan[n] = __ballot((h & 0x7fffu) > 0x7c00u);
+        any |= nan[n] != 0;
+      }
+      if (any) {
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+          if ((nan[n] >> lane) & 1) w[n / 2] &= n % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            bool hit = false;
+            for (int n = 0; n < 8; ++n)
+              for (int jj = 0; jj < 4; ++jj)
+                hit |= 4 * j + i < F::NG && ((nan[n] >> (16 * jj + 4 * j + i)) & 1) &&
+                       pos + 16 * (n / 4) + 4 * jj + n % 4 <= q.limit[rt];
+            if (hit) st.tail[rt][i] = __builtin_nanf("");
+          }
+        }
+      }
+    }
+  }
+  const half8 last = as_half8(w[0], w[1], w[2], w[3]);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    st.tail[rt] = mfma(last, ph[rt], st.tail[rt]);
+    if constexpr (kFine) st.tail[rt] = mfma(last, pl[rt], st.tail[rt]);
+  }
+  add_values<D, RT, 0>(x, ph, pl, kFine, st);
+}
+
+// Component `row` (0..15) of this lane's column of a 16x16 tile.
+__device__ inline float tile_row(const f32x4& t, int row, int lane) {
+  const int from = (row / 4) * 16 + lane % 16;
+  float v = 0.0f;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const float x = __shfl(t[c], from);
+    if (row % 4 == c) v = x;
+  }
+  return v;
+}
+
+// ---- shares of the row of units ---------------------------------------------------
+
+constexpr int rows_of(int RT) { return 16 * RT; }
+constexpr size_t record_floats(int D, int rows) { return static_cast<size_t>(rows) * (D + 2); }
+
+struct Share {
+  int64_t units;   // of the whole launch
+  int64_t groups;  // workgroups that take part
+  __device__ inline int64_t begin(int64_t w) const { return units * w / groups; }
+  __device__ inline int64_t owner(int64_t u) const { return ((u + 1) * groups - 1) / units; }
+};
+
+template <int NC>
+struct CombineSmem {
+  static constexpr int kChunk = NC < 8 ? NC : 8;
+  float m[kWaves][16];
+  float l[kWaves][16];
+  float acc[kWaves][kChunk * 4][kWave];
+};
+
+__device__ inline void store_out(const Params& p, int64_t token, int head, int D, int ch, const float* x, int n) {
+  const int64_t at = (token * p.query_heads + head) * D + ch;
+  if (n == 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x[i];
+    store8(p.out, at, p.type, v);
+  } else if (p.type == kF32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+        make_uint2(pack2(x[0], x[1], p.type), pack2(x[2], x[3], p.type));
+  }
+}
+
+struct Target {
+  int64_t token0;  // first query row of the sequence
+  int n_tokens;
+  int head0;       // first query head
+  int row0;        // first row of the tile (row = token * group + head)
+};
+
+template <int D, int RT, bool kFine, bool kCausal>
+__global__ __launch_bounds__(kThreads, RT == 1 && D <= 128 ? 2 : 1) void kv4_attention_kernel(const Params p) {
+  using F = Format<D>;
+  constexpr int kRows = rows_of(RT);
+  constexpr int kRecFloats = static_cast<int>(record_floats(D, kRows));
+  __shared__ CombineSmem<F::NC> cs;
+  __shared__ int64_t s_sum[kThreads + 1];
+  __shared__ int s_last;
+  const int tid = threadIdx.x;
+  const int wave = tid / kWave;
+  const int lane = tid % kWave;
+  const int r = lane % 16, j = lane / 16;
+  const int64_t w = blockIdx.x;
+
+  // ---- the units of the launch, and where this workgroup's share begins ----
+  // A list has at least one unit, so that an empty one is written too.
+  Share sh{0, 0};
+  const int lists = kCausal ? 0 : p.batch * p.select_groups;
+  const int per = (lists + kThreads - 1) / kThreads;
+  if constexpr (kCausal) {
+    sh.units = p.tile_info[1] * p.kv_heads;
+    if (sh.units <= 0) return;
+  } else {
+    int64_t mine = 0;
+    for (int s = tid * per; s < min((tid + 1) * per, lists); ++s)
+      mine += static_cast<int64_t>(max(decode_list(p, s / p.select_groups, s % p.select_groups).total, 1)) * p.kv_per_sel;
+    int64_t run = mine;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+      const int64_t x = __shfl_up(run, d);
+      if (lane >= d) run += x;
+    }
+    __shared__ int64_t s_wave[kWaves];
+    if (lane == kWave - 1) s_wave[wave] = run;
+    __syncthreads();
+    int64_t before = 0;
+    for (int i = 0; i < kWaves; ++i) {
+      if (i < wave) before += s_wave[i];
+      sh.units += s_wave[i];
+    }
+    s_sum[tid] = before + run - mine;
+    if (tid == 0) s_sum[kThreads] = sh.units;
+    __syncthreads();
+  }
+  sh.groups = min<int64_t>(gridDim.x, max<int64_t>(1, sh.units / kMinUnits));
+  if (w >= sh.groups) return;
+  int64_t u = sh.begin(w);
+  const int64_t end = sh.begin(w + 1);
+
+  // the list (decode: of one selection group's heads) or tile that holds u
+  int64_t base = 0;  // units before it
+  int s = 0;
+  if constexpr (kCausal) {
+    const int64_t at = u % p.tile_info[1];
+    int lo = 0, hi = static_cast<int>(p.tile_info[0]);
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (p.tile_first[mid] <= at) lo = mid;
+      else hi = mid;
+    }
+    s = lo;
+  } else {
+    int lo = 0, hi = kThreads;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (s_sum[mid] <= u) lo = mid;
+      else hi = mid;
+    }
+    s = lo * per;
+    base = s_sum[lo];
+  }
+
+  while (u < end) {
+    // ---- the list, its rows, and this share's pages [p0, p1) of it ----
+    int b, h;
+    List L;
+    int64_t list_first;  // unit of the list's first page
+    int pages;           // units of the list
+    Target tg;
+    int64_t limit0 = 0;
+    if constexpr (kCausal) {
+      const int64_t per_head = p.tile_info[1];
+      h = static_cast<int>(u / per_head);
+      const int4 t = p.tiles[s];
+      b = t.x;
+      pages = t.z;
+      list_first = h * per_head + p.tile_first[s];
+      tg.token0 = p.query_start[b];
+      tg.n_tokens = p.query_start[b + 1] - p.query_start[b];
+      tg.row0 = t.y;
+      const int64_t len = p.seq_len[b];
+      limit0 = len - tg.n_tokens;
+      L = List{nullptr, len, 0, 0, static_cast<int>((len + kPageTokens - 1) / kPageTokens)};
+    } else {
+      for (;;) {
+        b = s / p.select_groups;
+        L = decode_list(p, b, s % p.select_groups);
+        pages = max(L.total, 1);
+        if (u < base + static_cast<int64_t>(pages) * p.kv_per_sel) break;
+        base += static_cast<int64_t>(pages) * p.kv_per_sel;
+        ++s;
+      }
+      const int64_t k = (u - base) / pages;
+      h = (s % p.select_groups) * p.kv_per_sel + static_cast<int>(k);
+      list_first = base + k * pages;
+      tg.token0 = b;
+      tg.n_tokens = 1;
+      tg.row0 = 0;
+    }
+    tg.head0 = h * p.group;
+    const int p0 = static_cast<int>(u - list_first);
+    const int p1 = static_cast<int>(min<int64_t>(pages, p0 + (end - u)));
+
+    Rows<D, RT, kFine> q;
+    load_rows<D, RT, kFine>(p, q, tg.token0, tg.n_tokens, tg.head0, tg.row0, limit0, lane);
+    State<D, RT> st;
+    st.reset();
+    const int64_t first_limit = limit0 + tg.row0 / p.group;
+    const int64_t head_off = static_cast<int64_t>(h) * F::kRecord;
+    const int64_t page_bytes = static_cast<int64_t>(p.kv_heads) * F::kRecord;
+
+    // A lane looks up one of the wave's next 64 pages, so that the chain
+    // selected id -> table -> record is walked once for all of them.
+    for (int at = p0 + wave; at < p1; at += kWaves * kWave) {
+      const int mine = at + kWaves * lane;
+      PageRef ref{0, 0};
+      if (mine < p1) ref = resolve(p, b, L, mine);
+      const int n = min(kWave, (p1 - at + kWaves - 1) / kWaves);
+      for (int k = 0; k < n; ++k) {
+        const int valid = __builtin_amdgcn_readlane(ref.valid, k);
+        if (valid <= 0) continue;
+        const int64_t page = __builtin_amdgcn_readlane(ref.page, k);
+        Record<D> x;
+        load_record<D>(p.pool + page * page_bytes + head_off, lane, x);
+        attend<D, RT, kFine, kCausal>(x, valid, static_cast<int64_t>(at + kWaves * k) * kPageTokens, first_limit, q, st,
+                                      lane);
+      }
+    }
+
+    // ---- the waves' states, then the shares' records ----
+    const bool whole = p0 == 0 && p1 == pages;
+    const int64_t w0 = sh.owner(list_first), w1 = sh.owner(list_first + pages - 1);
+    float* rec = p.records + (2 * w + (p0 == 0 ? 1 : 0)) * static_cast<int64_t>(kRecFloats);
+    const int live_rows = min(kRows, tg.n_tokens * p.group - tg.row0);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float l = tile_row(st.tail[rt], F::NG, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float add = tile_row(st.tail[rt], (4 * j + i) * F::NC / 32, lane);
+#pragma unroll
+        for (int n = 0; n < F::NC; ++n) st.acc[rt][n][i] += add;
+      }
+      __syncthreads();  // the last round's readers are done
+      if (j == 0) {
+        cs.m[wave][r] = st.m[rt];
+        cs.l[wave][r] = l;
+      }
+      __syncthreads();
+      float top = kNegInf, sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) top = fmaxf(top, cs.m[i][r]);
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i)
+        if (cs.m[i][r] != kNegInf || cs.l[i][r] != 0.0f)
+          sum = __builtin_fmaf(cs.l[i][r], cs.m[i][r] == top ? 1.0f : __builtin_amdgcn_exp2f(cs.m[i][r] - top), sum);
+      const float f = st.m[rt] == top ? 1.0f : __builtin_amdgcn_exp2f(st.m[rt] - top);
+      const int row = rt * 16 + r;
+      const int token = (tg.row0 + row) / p.group, qh = tg.head0 + (tg.row0 + row) % p.group;
+      constexpr int kChunk = CombineSmem<F::NC>::kChunk;
+#pragma unroll
+      for (int c = 0; c < F::NC / kChunk; ++c) {
+        if (c) __syncthreads();
+#pragma unroll
+        for (int n = 0; n < kChunk; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) cs.acc[wave][n * 4 + i][lane] = st.acc[rt][c * kChunk + n][i] * f;
+        __syncthreads();
+        if (row < live_rows) {  // wave i adds up channels (4j + i) NC ..
+          float x[kChunk];
+#pragma unroll
+          for (int n = 0; n < kChunk; ++n) {
+            x[n] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) x[n] += cs.acc[v][n * 4 + wave][lane];
+          }
+          const int ch = (4 * j + wave) * F::NC + c * kChunk;
+          if (whole) {
+#pragma unroll
+            for (int n = 0; n < kChunk; ++n) x[n] = sum == 0.0f ? 0.0f : x[n] / sum;
+            store_out(p, tg.token0 + token, qh, D, ch, x, kChunk);
+          } else {
+#pragma unroll
+            for (int n = 0; n < kChunk; ++n) store_agent(rec + 2 * kRows + row * D + ch + n, x[n]);
+            if (c == 0 && wave == 0 && j == 0) {
+              store_agent(rec + 2 * row, top);
+              store_agent(rec + 2 * row + 1, sum);
+            }
+          }
+        }
+      }
+    }
+    if (!whole && last_arrival(p.arrive + w0, static_cast<int>(w1 - w0 + 1), &s_last)) {
+      const int shares = static_cast<int>(w1 - w0 + 1);
+      const float* first = p.records + (2 * w0 + 1) * static_cast<int64_t>(kRecFloats);
+      const auto record = [&](int i) { return i == 0 ? first : p.records + 2 * (w0 + i) * static_cast<int64_t>(kRecFloats); };
+      for (int e = tid; e < live_rows * (D / 4); e += kThreads) {
+        const int row = e / (D / 4), ch = e % (D / 4) * 4;
+        float top = kNegInf;
+        for (int i = 0; i < shares; ++i) top = fmaxf(top, load_agent(record(i) + 2 * row));
+        float sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < shares; ++i) {
+          const float* y = record(i);
+          const float m = load_agent(y + 2 * row), l = load_agent(y + 2 * row + 1);
+          const float f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+          sum = __builtin_fmaf(l, f, sum);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) x[n] = __builtin_fmaf(load_agent(y + 2 * kRows + row * D + ch + n), f, x[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) x[n] = sum == 0.0f ? 0.0f : x[n] / sum;
+        store_out(p, tg.token0 + (tg.row0 + row) / p.group, tg.head0 + (tg.row0 + row) % p.group, D, ch, x, 4);
+      }
+    }
+
+    u = list_first + p1;
+    if constexpr (kCausal) {
+      if (p1 == pages && ++s == static_cast<int>(p.tile_info[0])) s = 0;
+    }
+  }
+}
+
+// ---- the tiles of a ragged batch of query tokens ------------------------------------
+// Tile: `rows` rows (token * group + head) of one sequence, for every KV head.
+// Its pages end with the last one that its last row sees.  One workgroup.
+constexpr int kTileThreads = 1024;
+
+__global__ __launch_bounds__(kTileThreads) void tiles_kernel(const Params p, int rows) {
+  __shared__ int32_t before[kTileThreads + 1];
+  __shared__ int64_t s_wave[kTileThreads / kWave];
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int per = (p.batch + kTileThreads - 1) / kTileThreads;
+  const auto tokens_of = [&](int b) {
+    const int64_t a = p.query_start[b], z = p.query_start[b + 1];
+    return a >= 0 && z >= a && z <= p.tokens ? static_cast<int>(z - a) : 0;
+  };
+  const auto tiles_of = [&](int b) {
+    return static_cast<int>((static_cast<int64_t>(tokens_of(b)) * p.group + rows - 1) / rows);
+  };
+  const auto scan = [&](int64_t mine, int64_t& total) {
+    int64_t run = mine;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+      const int64_t x = __shfl_up(run, d);
+      if (lane >= d) run += x;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) s_wave[wave] = run;
+    __syncthreads();
+    int64_t pre = 0;
+    total = 0;
+    for (int i = 0; i < kTileThreads / kWave; ++i) {
+      if (i < wave) pre += s_wave[i];
+      total += s_wave[i];
+    }
+    return pre + run - mine;
+  };
+
+  // Starts that do not ascend within the rows make sequences share rows:
+  // then no tile is attended.
+  int64_t mine = 0;
+  bool bad = false;
+  for (int b = tid * per; b < min((tid + 1) * per, p.batch); ++b) {
+    const int64_t a = p.query_start[b], z = p.query_start[b + 1];
+    bad |= a < 0 || z < a || z > p.tokens;
+    if (tokens_of(b) > p.seq_len[b]) flag_status(p.status, kStatusBadLength);
+    mine += tiles_of(b);
+  }
+  int64_t tiles;
+  before[tid] = static_cast<int32_t>(min<int64_t>(scan(mine, tiles), INT32_MAX));
+  if (tid == 0) before[kTileThreads] = static_cast<int32_t>(min<int64_t>(tiles, INT32_MAX));
+  if (__syncthreads_or(bad)) {
+    tiles = 0;
+    if (tid == 0) flag_status(p.status, kStatusBadLength);
+  }
+  int64_t units = 0;
+  for (int64_t x0 = 0; x0 < tiles; x0 += kTileThreads) {
+    const int64_t x = x0 + tid;
+    int b = 0, row0 = 0, pages = 0;
+    if (x < tiles) {
+      int lo = 0, hi = kTileThreads;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (before[mid] <= x) lo = mid;
+        else hi = mid;
+      }
+      b = lo * per;
+      int64_t at = before[lo];
+      for (int n = tiles_of(b); x >= at + n; n = tiles_of(b)) {
+        at += n;
+        ++b;
+      }
+      row0 = static_cast<int>(x - at) * rows;
+      const int n = tokens_of(b);
+      const int last = min((row0 + rows - 1) / p.group, n - 1);
+      const int64_t limit = static_cast<int64_t>(p.seq_len[b]) - n + last;
+      pages = limit < 0 ? 1 : static_cast<int>(limit / kPageTokens) + 1;
+    }
+    int64_t sum;
+    const int64_t pre = scan(pages, sum);
+    if (x < tiles) {
+      p.tiles[x] = make_int4(b, row0, pages, 0);
+      p.tile_first[x] = units + pre;
+    }
+    units += sum;
+  }
+  if (tid == 0) {
+    p.tile_info[0] = tiles;
+    p.tile_info[1] = units;
+  }
+}
+
+// ---- launch ----------------------------------------------------------------------
+
+int grid_groups() { return std::min(kMaxGroups, compute_units() * kGroupsPerCu); }
+
+// Rows of a workgroup's tile: one token a sequence has `group` rows.
+// Two tiles of 16 rows fit the registers up to head_dim 128.
+int row_tiles(bool prompt, int head_dim) { return prompt && head_dim <= 128 ? 2 : 1; }
+
+int64_t max_tiles(int64_t batch, int64_t tokens, int group, int rows) {
+  return tokens * group / rows + std::min(batch, tokens) + 1;
+}
+
+struct Layout {
+  size_t records, info, first, tiles, bytes;
+};
+
+Layout layout(int64_t batch, int64_t tokens, int group, int head_dim, int RT) {
+  Layout l{};
+  const size_t counters = kMaxGroups * sizeof(int32_t);
+  const int64_t tiles = max_tiles(batch, tokens, group, rows_of(RT));
+  l.records = counters;
+  l.info = l.records + 2 * static_cast<size_t>(grid_groups()) * record_floats(head_dim, rows_of(RT)) * sizeof(float);
+  l.info = (l.info + 255) / 256 * 256;
+  l.first = l.info + 256;
+  l.tiles = (l.first + tiles * sizeof(int64_t) + 255) / 256 * 256;
+  l.bytes = l.tiles + tiles * sizeof(int4);
+  return l;
+}
+
+template <int D, int RT, bool kCausal>
+void launch_typed(const Params& p, bool fine, hipStream_t stream) {
+  const dim3 grid(grid_groups());
+  if (fine)
+    hipLaunchKernelGGL((kv4_attention_kernel<D, RT, true, kCausal>), grid, dim3(kThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL((kv4_attention_kernel<D, RT, false, kCausal>), grid, dim3(kThreads), 0, stream, p);
+}
+
+template <int D>
+void launch_dim(const Params& p, bool fine, hipStream_t stream) {
+  if (p.query_start)
+    launch_typed<D, D <= 128 ? 2 : 1, true>(p, fine, stream);
+  else
+    launch_typed<D, 1, false>(p, fine, stream);
+}
+
+}  // namespace
+
+size_t kv4_attention_workspace_bytes(int32_t batch, int32_t query_heads, int32_t kv_heads, int32_t head_dim,
+                                     int64_t tokens) {
+  size_t bytes = 0;  // either call's
+  for (int RT = 1; RT <= 2; ++RT)
+    bytes = std::max(bytes, layout(batch, tokens, query_heads / kv_heads, head_dim, RT).bytes);
+  return bytes;
+}
+
+hipError_t launch_kv4_attention(const Kv4AttnLaunch& a, hipStream_t stream) {
+  Params p{};
+  p.pool = a.pool;
+  p.table = a.table;
+  p.seq_len = a.seq_len;
+  p.sealed = a.sealed;
+  p.selected = a.selected;
+  p.counts = a.counts;
+  p.query_start = a.query_start;
+  p.query = a.query;
+  p.out = a.out;
+  p.status = a.status;
+  p.num_pages = a.num_pages;
+  p.q_stride = a.q_stride;
+  p.tokens = a.tokens;
+  p.batch = a.batch;
+  p.table_stride = a.table_stride;
+  p.sel_stride = a.sel_stride;
+  p.select_groups = a.selected ? a.select_groups : 1;
+  p.kv_per_sel = a.kv_heads / p.select_groups;
+  p.query_heads = a.query_heads;
+  p.kv_heads = a.kv_heads;
+  p.group = a.query_heads / a.kv_heads;
+  p.type = a.type;
+  p.qscale = a.scale * kLog2e;
+  const int RT = row_tiles(a.query_start != nullptr, a.head_dim);
+  const Layout l = layout(a.batch, a.tokens, p.group, a.head_dim, RT);
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  p.arrive = reinterpret_cast<int32_t*>(ws);
+  p.records = reinterpret_cast<float*>(ws + l.records);
+  p.tile_info = reinterpret_cast<int64_t*>(ws + l.info);
+  p.tile_first = reinterpret_cast<int64_t*>(ws + l.first);
+  p.tiles = reinterpret_cast<int4*>(ws + l.tiles);
+  if (a.query_start) {
+    hipLaunchKernelGGL(tiles_kernel, dim3(1), dim3(kTileThreads), 0, stream, p, rows_of(RT));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  const bool fine = a.type == kF32;
+  if (a.head_dim == 64) launch_dim<64>(p, fine, stream);
+  if (a.head_dim == 128) launch_dim<128>(p, fine, stream);
+  if (a.head_dim == 256) launch_dim<256>(p, fine, stream);
+  return hipGetLastError();
+}
+
+}  // namespace sa

@@ -363,4 +363,118 @@ hipError_t launch_fill_from_host(uint16_t* pool, int64_t page_bytes, int64_t num
 hipError_t launch_xor_bytes(const uint8_t* input, uint8_t* output, uint64_t bytes, uint8_t mask,
                             hipStream_t stream);
 
+// ---- pages handed out and taken back (page_table.hip) -----------------------
+struct ReserveLaunch {
+  int32_t* table;
+  const int32_t* seq_len;
+  const int32_t* new_tokens;
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t* query_start;
+  int32_t* slots;
+  int32_t* positions;  // or null
+  int32_t* seq_len_out;
+  int32_t* free_count_out;
+  int32_t* status;
+  int64_t num_pages;
+  int32_t batch;
+  int32_t table_stride;
+  int32_t max_tokens;
+  bool in_place;  // seq_len_out or free_count_out is its input
+};
+hipError_t launch_reserve_tokens(const ReserveLaunch& a, hipStream_t stream);
+
+struct ReleaseLaunch {
+  const int32_t* table;
+  const int32_t* seq_len;
+  int32_t* sealed;
+  const int32_t* finished;
+  int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t* seq_len_out;
+  int32_t* free_count_out;
+  int32_t* status;
+  int64_t num_pages;
+  int32_t batch;
+  int32_t table_stride;
+  bool in_place;
+};
+hipError_t launch_release_sequences(const ReleaseLaunch& a, hipStream_t stream);
+
+// ---- the cache in 4 bits ------------------------------------------------------
+// tokens of k, v ([token][kv_heads][head_dim], `type` one of kv4::Type) to or
+// from their slots (kv4_store.hip)
+struct Kv4RowsLaunch {
+  uint8_t* pool;
+  void* k;
+  void* v;
+  const int32_t* slots;
+  int32_t* status;
+  int64_t num_pages;
+  int64_t k_stride;
+  int64_t v_stride;
+  int32_t tokens;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t type;
+  bool load;
+};
+hipError_t launch_kv4_rows(const Kv4RowsLaunch& a, hipStream_t stream);
+
+struct Kv4SealLaunch {
+  uint8_t* pool;
+  const int32_t* table;
+  int32_t* seq_len;
+  int32_t* sealed;
+  int32_t* generation;
+  float* reps;
+  int32_t* status;
+  const void* k;  // append: [batch][kv_heads][head_dim]
+  const void* v;
+  int64_t num_pages;
+  int64_t k_stride;
+  int64_t v_stride;
+  int32_t batch;
+  int32_t table_stride;
+  int32_t kv_heads;
+  int32_t rep_heads;
+  int32_t rep_stride;
+  int32_t local_tokens;
+  int32_t head_dim;
+  int32_t type;
+};
+hipError_t launch_kv4_append_seal(const Kv4SealLaunch& a, hipStream_t stream);
+hipError_t launch_kv4_seal(const Kv4SealLaunch& a, hipStream_t stream);
+
+// Attention over the 4-bit pages (kv4_attention.hip).
+struct Kv4AttnLaunch {
+  const uint8_t* pool;
+  const int32_t* table;
+  const int32_t* seq_len;
+  const int32_t* sealed;
+  const int32_t* selected;     // decode: null for every page
+  const int32_t* counts;
+  const int32_t* query_start;  // prompt: [batch + 1]; null for one token a sequence
+  const void* query;           // [tokens][query_heads][head_dim]
+  void* out;
+  void* workspace;             // kv4_attention_workspace_bytes(), its counters zeroed once
+  int32_t* status;
+  int64_t num_pages;
+  int64_t q_stride;            // elements between tokens of the query
+  int32_t tokens;
+  int32_t batch;
+  int32_t table_stride;
+  int32_t sel_stride;
+  int32_t select_groups;
+  int32_t query_heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t type;
+  float scale;
+};
+constexpr int kKv4MaxGroup = 16;  // query heads per KV head: rows of a matrix-core tile
+size_t kv4_attention_workspace_bytes(int32_t batch, int32_t query_heads, int32_t kv_heads, int32_t head_dim,
+                                     int64_t tokens);
+hipError_t launch_kv4_attention(const Kv4AttnLaunch& a, hipStream_t stream);
+
 }  // namespace sa

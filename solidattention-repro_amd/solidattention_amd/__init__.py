@@ -135,6 +135,16 @@ EXPORTS = {
     "sa_hip_fill_pages_async": (C.c_int, [_P, _I64, _P, _P, _P, _I32, _P, _P]),
     "sa_hip_fill_pages_gather_async": (C.c_int, [_P, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _P, _P]),
     "sa_hip_stream_wait_event": (C.c_int, [_P, _P]),
+    "sa_hip_reserve_tokens": (C.c_int, [_KV, _P, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _P]),
+    "sa_hip_release_sequences": (C.c_int, [_KV, _P, _P, _P, _P, _P, _P, _P]),
+    "sa_hip_kv4_page_bytes": (_SZ, [_I32, _I32]),
+    "sa_hip_kv4_store": (C.c_int, [_KV, _P, _P, _I32, _I64, _I64, _P, _I32, _P, _P]),
+    "sa_hip_kv4_load": (C.c_int, [_KV, _P, _P, _I32, _I64, _I64, _P, _I32, _P, _P]),
+    "sa_hip_kv4_append_seal": (C.c_int, [_KV, _P, _P, _I32, _I64, _I64, _I32, _P, _P]),
+    "sa_hip_kv4_seal": (C.c_int, [_KV, _I32, _P, _P]),
+    "sa_hip_kv4_attention_workspace_bytes": (_SZ, [_KV, _I32]),
+    "sa_hip_kv4_decode_attention": (C.c_int, [_KV, _P, _I32, _I64, _P, _P, _I32, _I32, _F, _P, _P, _SZ, _P, _P]),
+    "sa_hip_kv4_prompt_attention": (C.c_int, [_KV, _P, _I32, _I64, _P, _I32, _F, _P, _P, _SZ, _P, _P]),
     "sa_hip_fill_synthetic_f16": (C.c_int, [_P, _I64, C.c_uint64, C.c_uint64, _P]),
     "sa_hip_fill_synthetic_f32": (C.c_int, [_P, _I64, C.c_uint64, C.c_uint64, _P]),
 }
@@ -795,6 +805,255 @@ def local_causal_representatives(prompt_queries, kv16, tokens, query_heads, kv_h
         _ptr(vals), _ptr(offs), _ptr(reps), rep_stride, _ptr(received), _ptr(ws), nbytes, _stream(stream)),
         "local_causal_representatives")
     return vals, offs
+
+
+# --------------------------------------------------------------------------
+# pages handed out on the GPU, and the cache in 4 bits
+# --------------------------------------------------------------------------
+
+POOL_KV4 = 0x4B563434
+F32, F16, BF16 = 0, 1, 2
+
+
+class _On:
+    """The device of a call's tensors made current, and the stream that the call runs on (the given one, or that
+    device's current one); what is allocated inside belongs to that stream."""
+
+    def __init__(self, device, stream=None):
+        import torch
+        self.device = torch.cuda.device(device)
+        self.given = stream
+        self.place = device
+
+    def __enter__(self):
+        import torch
+        self.device.__enter__()
+        s = self.given if self.given is not None else torch.cuda.current_stream(self.place)
+        self.scope = torch.cuda.stream(s)
+        self.scope.__enter__()
+        return C.c_void_p(s.cuda_stream)
+
+    def __exit__(self, *a):
+        self.scope.__exit__(*a)
+        return self.device.__exit__(*a)
+
+
+def _type_of(x, what):
+    import torch
+    types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    if x.dtype not in types:
+        raise ValueError(f"{what}: {x.dtype} is not float32, float16 or bfloat16")
+    return types[x.dtype]
+
+
+def _heads_rows(x, heads, head_dim, what, device):
+    """Elements between the tokens of x [tokens][heads][head_dim], whose rows are whole."""
+    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != head_dim:
+        raise ValueError(f"{what}: shape {tuple(x.shape)} is not [tokens, {heads}, {head_dim}]")
+    if x.device != device:
+        raise ValueError(f"{what} is on {x.device}, the cache on {device}")
+    if x.stride(2) != 1 or (heads > 1 and x.stride(1) != head_dim):
+        raise ValueError(f"{what}: a token's heads must be contiguous (strides {x.stride()})")
+    if x.shape[0] <= 1:
+        return heads * head_dim
+    if x.stride(0) < heads * head_dim:
+        raise ValueError(f"{what}: rows overlap (strides {x.stride()})")
+    return x.stride(0)
+
+
+def _ints(x, count, what, device):
+    import torch
+    if x.dtype != torch.int32 or not x.is_contiguous() or x.numel() < count:
+        raise ValueError(f"{what} must be a contiguous int32 tensor of at least {count} elements")
+    if x.device != device:
+        raise ValueError(f"{what} is on {x.device}, the cache on {device}")
+    return x
+
+
+class PagedKV4(PagedKV):
+    """PagedKV whose pages are held in 4 bits (the format in include/sa_hip.h): 5/16 of the bytes.
+
+    pool  uint8 [num_pages, kv_heads, 40 * head_dim], head_dim 64, 128 or 256
+
+    Selection (score_select and its other forms) takes it as it is; the pages are written and read by the kv4
+    functions.  generation, sealed and reps mean what they do in PagedKV."""
+
+    def __init__(self, batch, query_heads, kv_heads, table_stride, num_pages=None, rep_heads=None, rep_stride=None,
+                 head_dim=HEAD_DIM, device="cuda", pool=None):
+        import torch
+        pages = num_pages if num_pages is not None else batch * table_stride
+        if not lib().sa_hip_kv4_page_bytes(kv_heads, head_dim):
+            raise ValueError(f"no 4-bit pages of {kv_heads} heads and head_dim {head_dim} (64, 128 or 256)")
+        shape = (pages, kv_heads, 40 * head_dim)
+        if pool is None:
+            pool = torch.zeros(shape, dtype=torch.uint8, device=torch.device(device))
+        elif pool.dtype != torch.uint8 or tuple(pool.shape) != shape or not pool.is_contiguous():
+            raise ValueError(f"pool must be a contiguous uint8 tensor of shape {shape}")
+        super().__init__(batch, query_heads, kv_heads, table_stride, num_pages=pages, rep_heads=rep_heads,
+                         rep_stride=rep_stride, head_dim=head_dim, device=pool.device, pool=pool)
+
+    def struct(self) -> PagedKVStruct:
+        s = super().struct()
+        s.reserved = POOL_KV4
+        return s
+
+    @property
+    def page_bytes(self) -> int:
+        return self.kv_heads * 40 * self.head_dim
+
+
+def reserve_tokens(kv: PagedKV, new_tokens, free_pages, free_count, query_start, slots, positions=None,
+                   seq_len_out=None, free_count_out=None, status=None, stream=None):
+    """Pages for new_tokens[b] more tokens of each sequence, off the stack free_pages[:free_count] (int32
+    [num_pages], [1]), into kv.block_table; query_start [batch + 1], slots and positions [max_tokens] of the new
+    tokens (-1 behind the last).  seq_len_out and free_count_out default to kv.seq_len and free_count (in place).
+    All or nothing: where the pages, a table row or the slots do not suffice, status says so, query_start is 0, the
+    slots are -1 and nothing else changes."""
+    dev = kv.block_table.device
+    seq_len_out = kv.seq_len if seq_len_out is None else seq_len_out
+    free_count_out = free_count if free_count_out is None else free_count_out
+    _ints(kv.block_table, kv.batch * kv.table_stride, "block_table", dev)
+    for x, n, what in ((kv.seq_len, kv.batch, "seq_len"), (new_tokens, kv.batch, "new_tokens"),
+                       (free_pages, kv.num_pages, "free_pages"), (free_count, 1, "free_count"),
+                       (query_start, kv.batch + 1, "query_start"), (slots, 0, "slots"),
+                       (seq_len_out, kv.batch, "seq_len_out"), (free_count_out, 1, "free_count_out")):
+        _ints(x, n, what, dev)
+    if positions is not None:
+        _ints(positions, slots.numel(), "positions", dev)
+    s = kv.struct()
+    with _On(dev, stream) as st:
+        check(lib().sa_hip_reserve_tokens(C.byref(s), _ptr(new_tokens), _ptr(free_pages), _ptr(free_count),
+                                          slots.numel(), _ptr(query_start), _ptr(slots), _ptr(positions),
+                                          _ptr(seq_len_out), _ptr(free_count_out), _ptr(status), st),
+              "reserve_tokens")
+    return query_start, slots, positions
+
+
+def release_sequences(kv: PagedKV, finished, free_pages, free_count, seq_len_out=None, free_count_out=None,
+                      status=None, stream=None):
+    """The pages of the sequences with finished[b] != 0 (int32) go back onto the stack; their lengths and sealed
+    counts become 0.  In place unless seq_len_out and free_count_out are given."""
+    dev = kv.block_table.device
+    seq_len_out = kv.seq_len if seq_len_out is None else seq_len_out
+    free_count_out = free_count if free_count_out is None else free_count_out
+    _ints(kv.block_table, kv.batch * kv.table_stride, "block_table", dev)
+    for x, n, what in ((kv.seq_len, kv.batch, "seq_len"), (kv.sealed, kv.batch, "sealed"),
+                       (finished, kv.batch, "finished"), (free_pages, kv.num_pages, "free_pages"),
+                       (free_count, 1, "free_count"), (seq_len_out, kv.batch, "seq_len_out"),
+                       (free_count_out, 1, "free_count_out")):
+        _ints(x, n, what, dev)
+    s = kv.struct()
+    with _On(dev, stream) as st:
+        check(lib().sa_hip_release_sequences(C.byref(s), _ptr(finished), _ptr(free_pages), _ptr(free_count),
+                                             _ptr(seq_len_out), _ptr(free_count_out), _ptr(status), st),
+              "release_sequences")
+
+
+def _kv4_rows(kv, k, v, tokens):
+    dev = kv.pool.device
+    stride = [_heads_rows(x, kv.kv_heads, kv.head_dim, what, dev) for x, what in ((k, "k"), (v, "v"))]
+    if k.dtype != v.dtype or k.shape[0] != v.shape[0] or k.shape[0] < tokens:
+        raise ValueError(f"k and v must have one dtype and at least {tokens} tokens")
+    return _type_of(k, "k"), stride[0], stride[1]
+
+
+def kv4_store(kv: PagedKV4, k, v, slots, status=None, stream=None):
+    """k, v [tokens, kv_heads, head_dim] (float32, float16 or bfloat16; the tokens may be strided, as parts of a fused
+    projection) into the 4-bit pages at slots [tokens] (int32, page * 32 + offset); a negative slot is passed over."""
+    n = slots.numel()
+    type_, ks, vs = _kv4_rows(kv, k, v, n)
+    _ints(slots, n, "slots", kv.pool.device)
+    s = kv.struct()
+    with _On(kv.pool.device, stream) as st:
+        check(lib().sa_hip_kv4_store(C.byref(s), _ptr(k), _ptr(v), type_, ks, vs, _ptr(slots), n, _ptr(status), st),
+              "kv4_store")
+
+
+def kv4_load(kv: PagedKV4, slots, k, v, status=None, stream=None):
+    """The values that the cache holds at slots, into k and v (rows of negative slots stay as they are)."""
+    n = slots.numel()
+    type_, ks, vs = _kv4_rows(kv, k, v, n)
+    _ints(slots, n, "slots", kv.pool.device)
+    s = kv.struct()
+    with _On(kv.pool.device, stream) as st:
+        check(lib().sa_hip_kv4_load(C.byref(s), _ptr(k), _ptr(v), type_, ks, vs, _ptr(slots), n, _ptr(status), st),
+              "kv4_load")
+    return k, v
+
+
+def kv4_append_seal(kv: PagedKV4, k, v, local_tokens, status=None, stream=None):
+    """append_seal on 4-bit pages: one token per sequence, k, v [batch, kv_heads, head_dim]."""
+    type_, ks, vs = _kv4_rows(kv, k, v, kv.batch)
+    s = kv.struct()
+    with _On(kv.pool.device, stream) as st:
+        check(lib().sa_hip_kv4_append_seal(C.byref(s), _ptr(k), _ptr(v), type_, ks, vs, local_tokens, _ptr(status),
+                                           st), "kv4_append_seal")
+
+
+def kv4_seal(kv: PagedKV4, local_tokens, status=None, stream=None):
+    """seal on 4-bit pages (after kv4_store wrote a prompt and its lengths were set)."""
+    s = kv.struct()
+    with _On(kv.pool.device, stream) as st:
+        check(lib().sa_hip_kv4_seal(C.byref(s), local_tokens, _ptr(status), st), "kv4_seal")
+
+
+def kv4_attention_workspace(kv: PagedKV4, query_tokens=None):
+    """A zeroed workspace for kv4_decode_attention and kv4_prompt_attention of up to query_tokens rows (the batch when
+    None).  Calls that share one must not overlap; a captured graph keeps its own."""
+    import torch
+    n = int(lib().sa_hip_kv4_attention_workspace_bytes(C.byref(kv.struct()),
+                                                       kv.batch if query_tokens is None else query_tokens))
+    return torch.zeros(max(n, 16), dtype=torch.uint8, device=kv.pool.device)
+
+
+def _kv4_attention(kv, query, out, workspace):
+    import torch
+    stride = _heads_rows(query, kv.query_heads, kv.head_dim, "query", kv.pool.device)
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    elif out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous() or out.device != query.device:
+        raise ValueError("out must be contiguous, of the query's shape, dtype and device")
+    if workspace is None:
+        workspace = kv4_attention_workspace(kv, query.shape[0])
+    elif workspace.device != query.device or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous and on the query's device")
+    return stride, out, workspace, workspace.numel() * workspace.element_size()
+
+
+def kv4_decode_attention(kv: PagedKV4, query, scale, selected=None, counts=None, out=None, workspace=None,
+                         status=None, stream=None):
+    """Attention of one token a sequence, query [batch, query_heads, head_dim] (float32, float16 or bfloat16; out
+    has its type), over the 4-bit pages: the selected blocks (selected [batch, groups, stride] and counts, as
+    score_select gives them) and the tail, or the whole sequences when selected is None."""
+    if query.dim() != 3 or query.shape[0] != kv.batch:
+        raise ValueError(f"query: shape {tuple(query.shape)} does not hold one token for each of {kv.batch} sequences")
+    groups = sel_stride = 0
+    if selected is not None:
+        groups, sel_stride = selected.shape[1], selected.shape[2]
+        _ints(selected, kv.batch * groups * sel_stride, "selected", kv.pool.device)
+        _ints(counts, kv.batch * groups, "counts", kv.pool.device)
+    s = kv.struct()
+    with _On(kv.pool.device, stream) as st:
+        stride, out, workspace, nbytes = _kv4_attention(kv, query, out, workspace)
+        check(lib().sa_hip_kv4_decode_attention(
+            C.byref(s), _ptr(query), _type_of(query, "query"), stride, _ptr(selected), _ptr(counts), groups,
+            sel_stride, C.c_float(scale), _ptr(out), _ptr(workspace), nbytes, _ptr(status), st),
+            "kv4_decode_attention")
+    return out
+
+
+def kv4_prompt_attention(kv: PagedKV4, query, query_start, scale, out=None, workspace=None, status=None, stream=None):
+    """Causal attention of several tokens a sequence over the 4-bit pages, which hold them already: rows
+    [query_start[b], query_start[b + 1]) of query [tokens, query_heads, head_dim] are the last tokens of sequence b.
+    Rows outside every range are left as they are."""
+    _ints(query_start, kv.batch + 1, "query_start", kv.pool.device)
+    s = kv.struct()
+    with _On(kv.pool.device, stream) as st:
+        stride, out, workspace, nbytes = _kv4_attention(kv, query, out, workspace)
+        check(lib().sa_hip_kv4_prompt_attention(
+            C.byref(s), _ptr(query), _type_of(query, "query"), stride, _ptr(query_start), query.shape[0],
+            C.c_float(scale), _ptr(out), _ptr(workspace), nbytes, _ptr(status), st), "kv4_prompt_attention")
+    return out
 
 
 def gather_pages(pool, page_bytes, num_pages, pages, out, status=None, stream=None):
