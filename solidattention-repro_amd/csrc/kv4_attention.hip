@@ -7,10 +7,9 @@
 //
 // Everything runs on v_mfma_f32_16x16x32_f16, whose K is one group:
 //   scores   tile T: rows = tokens 16T.., columns = query rows.  The codes
-//            enter as 64 + c (the nibble moved into the mantissa of 64.0: one
-//            shift and one and-or for two), the accumulator starts at -64 sum
-//            q, and the group's sum takes its token's scale in fp32.  The
-//            minima are one more product: m_tg against the groups' sums of q.
+//            enter as FP16 integers and the group's sum takes its token's
+//            scale in fp32.  The minima are one more product: m_tg against
+//            the groups' sums of q.
 //   values   rows = channels, columns = query rows, products over tokens.
 //            The operand is c * s, exact in FP16 (7-bit scales); the minima
 //            and the denominator are one more product, with rows m_g and 1.
@@ -18,8 +17,8 @@
 // (query row, quarter of the tokens), which is the second product's operand.
 // fp32 queries and probabilities enter as a high and a low FP16 part (22
 // bits); 16-bit queries are exact in one part and the probabilities round to
-// FP16 (2^-11 relative).  Queries are scaled by a power of two per row, the
-// probabilities by 2^14: neither underflows in FP16 before 2^-38 of its largest.
+// FP16 (2^-11 relative).  Queries are scaled by a power of two per row, so that
+// none of their parts underflows before 2^-24 of the row's largest.
 //
 // Work is split by pages, not by lists: the pages of all (sequence, KV head)
 // lists form one row of units, and each workgroup takes an equal share of it,
@@ -42,12 +41,20 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kGroupsPerCu = 4;
 constexpr int kMaxGroups = 4096;   // workgroups, and arrival counters at the front of the workspace
 constexpr int kMinUnits = 8;       // pages a workgroup is worth starting for
 constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLowest = -3.0e38f;  // of masked scores: finite, so that a factor of 0 leaves no NaN
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kProbShift = 14.0f;  // probabilities are held times 2^14
+
+// Probabilities are held times 2^shift, against a maximum that may lag the
+// true one by `lag` (in exponents of 2): they stay below FP16's largest
+// number, and down to 2^-(25 + shift) of the row's largest they are not lost.
+// Without a lag every page's maximum would cross lanes and rescale the sums.
+template <bool kFine>
+constexpr float kShift = kFine ? 14.0f : 6.0f;
+template <bool kFine>
+constexpr float kLag = kFine ? 1.0f : 9.0f;
 
 struct Params {
   const uint8_t* pool;
@@ -150,7 +157,26 @@ __device__ inline PageRef resolve(const Params& p, int b, const List& L, int i) 
   return r;
 }
 
-// ---- a record in a wave's registers ----------------------------------------------
+// ---- a record in LDS -------------------------------------------------------------
+// A wave copies its next record from memory straight into its LDS slot while it
+// attends the present one out of registers: no registers are held in flight,
+// which leaves room for more waves.
+
+typedef const void __attribute__((address_space(1)))* GlobalPtr;
+typedef void __attribute__((address_space(3)))* LdsPtr;
+constexpr int kDmaNontemporal = 2;  // a record is read once
+
+template <int D>
+__device__ inline void fetch_record(const uint8_t* rec, uint8_t* slot, int lane) {
+  constexpr int kBytes = Format<D>::kRecord;
+#pragma unroll
+  for (int at = 0; at < kBytes; at += kWave * 16)
+    if (at + kWave * 16 <= kBytes || lane * 16 < kBytes - at)
+      __builtin_amdgcn_global_load_lds((GlobalPtr)(rec + at + lane * 16), (LdsPtr)(slot + at), 16, 0, kDmaNontemporal);
+}
+__device__ inline void wait_fetch() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// The slot may be fetched into once its reads have returned.
+__device__ inline void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 template <int D>
 struct Record {
@@ -164,35 +190,34 @@ struct Record {
 };
 
 template <int N>
-__device__ inline void load_words(const uint8_t* p, uint32_t* w) {
+__device__ inline void read_words(const uint8_t* p, uint32_t* w) {
   if constexpr (N == 1) {
-    w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   } else if constexpr (N == 2) {
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
     w[0] = x.x, w[1] = x.y;
   } else {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-      const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 4 * i));
+      const uint4 x = *reinterpret_cast<const uint4*>(p + 4 * i);
       w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
     }
   }
 }
 
 template <int D>
-__device__ inline void load_record(const uint8_t* rec, int lane, Record<D>& x) {
+__device__ inline void read_record(const uint8_t* slot, int lane, Record<D>& x) {
   using F = Format<D>;
   const int r = lane % 16, j = lane / 16;
 #pragma unroll
   for (int T = 0; T < 2; ++T) {
-    load_words<F::NG>(rec + (16 * T + r) * (D / 2) + j * F::NG * 4, x.kc[T]);
-    load_words<F::NC / 2>(rec + F::kValueCodes + ((T * 4 + j) * 16 + r) * 2 * F::NC, x.vc[T]);
-    load_words<F::NG * 2>(rec + F::kKeyScales + (T * 4 + j) * F::NG * 8, x.ks[T]);
-    load_words<F::NG / 2>(rec + F::kKeyMins + (16 * T + r) * F::NG * 2, x.km[T]);
+    read_words<F::NG / 2>(slot + F::kKeyMins + (16 * T + r) * F::NG * 2, x.km[T]);
+    read_words<F::NG>(slot + (16 * T + r) * (D / 2) + j * F::NG * 4, x.kc[T]);
+    read_words<F::NG * 2>(slot + F::kKeyScales + (T * 4 + j) * F::NG * 8, x.ks[T]);
+    read_words<F::NC / 2>(slot + F::kValueCodes + ((T * 4 + j) * 16 + r) * 2 * F::NC, x.vc[T]);
   }
-  load_words<4>(rec + F::kValueScales + (r * F::NC / 32 * 4 + j) * 16, x.vs);
-  load_words<4>(rec + F::kValueMins + (r % F::NG * 4 + j) * 16, x.vm);
+  read_words<4>(slot + F::kValueMins + (r % F::NG * 4 + j) * 16, x.vm);
+  read_words<4>(slot + F::kValueScales + (r * F::NC / 32 * 4 + j) * 16, x.vs);
 }
 
 __device__ inline half8 as_half8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -201,24 +226,30 @@ __device__ inline half8 as_half8(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 __device__ inline half2_t as_half2(uint32_t a) { return __builtin_bit_cast(half2_t, a); }
 __device__ inline uint32_t bits_of(half2_t a) { return __builtin_bit_cast(uint32_t, a); }
 
-// 8 nibbles as 64 + c, in the order (0,4), (1,5), (2,6), (3,7).
-__device__ inline half8 codes_plus64(uint32_t w) {
-  constexpr uint32_t kMask = 0x00F000F0u, kBase = 0x54005400u;  // 64.0: the mantissa's bits 4..7 count units
-  return as_half8(((w << 4) & kMask) | kBase, (w & kMask) | kBase, ((w >> 4) & kMask) | kBase,
-                  ((w >> 8) & kMask) | kBase);
+// x & mask | base in one instruction (the compiler splits it over two literals).
+__device__ inline uint32_t and_or(uint32_t x, uint32_t mask, uint32_t base) {
+  uint32_t d;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(d) : "v"(x), "s"(mask), "v"(base));
+  return d;
+}
+
+// Nibbles 0 and 1 of both halves as FP16 integers: moved into the mantissa of
+// 1024.0 (bits 0..3) or 64.0 (bits 4..7), which is then taken off (exact).
+__device__ inline half2_t low_nibbles(uint32_t w) { return as_half2(and_or(w, 0x000F000Fu, 0x64006400u)) - half2_t{1024, 1024}; }
+__device__ inline half2_t high_nibbles(uint32_t w) { return as_half2(and_or(w, 0x00F000F0u, 0x54005400u)) - half2_t{64, 64}; }
+
+// 8 nibbles in the order (0,4), (1,5), (2,6), (3,7).
+__device__ inline half8 key_codes(uint32_t w) {
+  return as_half8(bits_of(low_nibbles(w)), bits_of(high_nibbles(w)), bits_of(low_nibbles(w >> 8)),
+                  bits_of(high_nibbles(w >> 8)));
 }
 
 // Nibble n (0..3) of both halves as FP16 integers times the pair of scales
 // (exact: 4 + 7 bits).
 template <int N>
 __device__ inline uint32_t scaled_codes(uint32_t y, uint32_t scales) {
-  half2_t c;
   const uint32_t w = N < 2 ? y : y >> 8;
-  if constexpr (N % 2 == 0)
-    c = as_half2((w & 0x000F000Fu) | 0x64006400u) - half2_t{1024, 1024};
-  else
-    c = as_half2((w & 0x00F000F0u) | 0x54005400u) - half2_t{64, 64};
-  return bits_of(c * as_half2(scales));
+  return bits_of((N % 2 == 0 ? low_nibbles(w) : high_nibbles(w)) * as_half2(scales));
 }
 
 __device__ inline f32x4 mfma(half8 a, half8 b, f32x4 c) {
@@ -257,7 +288,6 @@ struct Rows {
   using F = Format<D>;
   half8 hi[RT][F::NG];
   half8 lo[RT][kFine ? F::NG : 1];
-  float base[RT][F::NG];  // -64 sum q of a group
   half8 sums[RT];         // operand of the minima
   float factor[RT];
   int64_t limit[RT];      // last position the row sees
@@ -282,16 +312,21 @@ __device__ inline void load_rows(const Params& p, Rows<D, RT, kFine>& q, int64_t
     for (int g = 0; g < F::NG; ++g) {
 #pragma unroll
       for (int n = 0; n < 8; ++n) x[g][n] = 0.0f;
-      if (live)
-        load8(p.query, (token0 + token) * p.q_stride + static_cast<int64_t>(head0 + row % p.group) * D + 32 * g + 8 * j,
-              p.type, x[g]);
+      const int64_t at =
+          (token0 + token) * p.q_stride + static_cast<int64_t>(head0 + row % p.group) * D + 32 * g + 8 * j;
+      if (live) {
+        if constexpr (kFine)
+          load8(p.query, at, kF32, x[g]);
+        else
+          load8(p.query, at, p.type == kF16 ? kF16 : kBF16, x[g]);
+      }
 #pragma unroll
       for (int n = 0; n < 8; ++n) top = fmaxf(top, fabsf(x[g][n]));
     }
     top = xor_max<32>(xor_max<16>(top));
     // the row's largest value into [1, 2): a power of two, exact
     const int e = top > 0.0f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
-    q.factor[rt] = ldexp2(p.qscale, e);
+    q.factor[rt] = ldexp2(fabsf(p.qscale), e);  // not negative: the scale's sign goes to q
     float sum[F::NG];
 #pragma unroll
     for (int g = 0; g < F::NG; ++g) {
@@ -300,7 +335,7 @@ __device__ inline void load_rows(const Params& p, Rows<D, RT, kFine>& q, int64_t
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
         const int c = n / 2 + (n % 2) * 4;  // operand order (0,4), (1,5), ...
-        const float v = ldexp2(x[g][c], -e);
+        const float v = ldexp2(p.qscale < 0.0f ? -x[g][c] : x[g][c], -e);
         hi[n] = static_cast<_Float16>(v);
         lo[n] = static_cast<_Float16>(v - static_cast<float>(hi[n]));
         s += static_cast<float>(hi[n]);
@@ -309,7 +344,6 @@ __device__ inline void load_rows(const Params& p, Rows<D, RT, kFine>& q, int64_t
       q.hi[rt][g] = hi;
       if constexpr (kFine) q.lo[rt][g] = lo;
       s = xor_sum<32>(xor_sum<16>(s));
-      q.base[rt][g] = -64.0f * s;
       sum[g] = s;
     }
     // products of the minima: NG slots of high parts, NG of low ones
@@ -338,7 +372,9 @@ struct State {
   float m[RT];
   f32x4 acc[RT][F::NC];  // channel (4j + i) NC + n of query row r
   f32x4 tail[RT];        // rows 0..NG-1: minima of each group; row NG: the denominator
+  bool huge;             // some maximum's rounding is no small change (the same in every lane)
   __device__ inline void reset() {
+    huge = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       m[rt] = kNegInf;
@@ -396,12 +432,11 @@ __device__ inline void attend(Record<D>& x, int valid, int64_t pos, int64_t firs
     for (int rt = 0; rt < RT; ++rt) z[rt][T] = mfma(mins, q.sums[rt], f32x4{0, 0, 0, 0});
 #pragma unroll
     for (int g = 0; g < F::NG; ++g) {
-      const half8 k = codes_plus64(x.kc[T][g]);
+      const half8 k = key_codes(x.kc[T][g]);
       const uint32_t s01 = x.ks[T][2 * g], s23 = x.ks[T][2 * g + 1];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float b = q.base[rt][g];
-        f32x4 d = mfma(k, q.hi[rt][g], f32x4{b, b, b, b});
+        f32x4 d = mfma(k, q.hi[rt][g], f32x4{0, 0, 0, 0});
         if constexpr (kFine) d = mfma(k, q.lo[rt][g], d);
         z[rt][T][0] = __builtin_fmaf(lo_h2f(s01), d[0], z[rt][T][0]);
         z[rt][T][1] = __builtin_fmaf(hi_h2f(s01), d[1], z[rt][T][1]);
@@ -412,36 +447,41 @@ __device__ inline void attend(Record<D>& x, int valid, int64_t pos, int64_t firs
   }
 
   half8 ph[RT], pl[RT];
+  const bool masked = valid < kPageTokens || cut;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    float e[8];
-#pragma unroll
-    for (int n = 0; n < 8; ++n) e[n] = z[rt][n / 4][n % 4] * q.factor[rt];
-    if (valid < kPageTokens || cut) {
-      int seen = valid;
+    int seen = valid;
+    if (masked) {
       if (kCausal) {
         const int64_t left = q.limit[rt] - pos + 1;
         if (left < seen) seen = left < 0 ? 0 : static_cast<int>(left);
       }
 #pragma unroll
-      for (int n = 0; n < 8; ++n) e[n] = 16 * (n / 4) + 4 * j + n % 4 < seen ? e[n] : kNegInf;
+      for (int n = 0; n < 8; ++n)
+        z[rt][n / 4][n % 4] = 16 * (n / 4) + 4 * j + n % 4 < seen ? z[rt][n / 4][n % 4] : kLowest;
     }
-    float top = e[0];
+    float top = z[rt][0][0];
 #pragma unroll
-    for (int n = 1; n < 8; ++n) top = fmaxf(top, e[n]);
-    top = xor_max<32>(xor_max<16>(top));
-    if (__any(top > st.m[rt])) {
-      const bool up = top > st.m[rt];
-      const float f = up ? __builtin_amdgcn_exp2f(st.m[rt] - top) : 1.0f;
-      st.m[rt] = up ? top : st.m[rt];
+    for (int n = 1; n < 8; ++n) top = fmaxf(top, z[rt][n / 4][n % 4]);
+    top *= q.factor[rt];
+    if (__any(top > st.m[rt] + kLag<kFine>)) {
+      top = fmaxf(xor_max<32>(xor_max<16>(top)), st.m[rt]);
+      const float f = top > st.m[rt] ? __builtin_amdgcn_exp2f(st.m[rt] - top) : 1.0f;
+      st.m[rt] = top;
+      st.huge |= __any(!(fabsf(top) < 0x1p20f));
       st.tail[rt] *= f;
 #pragma unroll
       for (int n = 0; n < F::NC; ++n) st.acc[rt][n] *= f;
     }
-    const float off = (st.m[rt] == kNegInf ? 0.0f : st.m[rt]) - kProbShift;
+    const float off = kShift<kFine> - st.m[rt];
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      const float v = __builtin_amdgcn_exp2f(e[n] - off);
+      // one rounding for product and difference: the maximum's own rounding is
+      // the row's common factor, unless it passes the whole range of FP16
+      float x = __builtin_fmaf(z[rt][n / 4][n % 4], q.factor[rt], off);
+      if (st.huge) x = z[rt][n / 4][n % 4] * q.factor[rt] + off;
+      float v = __builtin_amdgcn_exp2f(x);
+      if (masked) v = 16 * (n / 4) + 4 * j + n % 4 < seen ? v : 0.0f;
       ph[rt][n] = static_cast<_Float16>(v);
       if constexpr (kFine) pl[rt][n] = static_cast<_Float16>(v - static_cast<float>(ph[rt][n]));
     }
@@ -462,28 +502,30 @@ __device__ inline void attend(Record<D>& x, int valid, int64_t pos, int64_t firs
   // reach the others, so it is taken out and added to the rows that see it.
   if constexpr (kCausal) {
     if (cut) {
-      uint64_t nan[8];
       bool any = false;
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
-        const uint16_t h = static_cast<uint16_t>(w[n / 2] >> (16 * (n % 2)));
-        nan[n] = __ballot((h & 0x7fffu) > 0x7c00u);
-        any |= nan[n] != 0;
+        const bool nan = ((w[n / 2] >> (16 * (n % 2))) & 0x7fffu) > 0x7c00u;
+        if (nan) w[n / 2] &= n % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+        any |= nan;
       }
-      if (any) {
+      if (__any(any)) {
+#pragma unroll 1
+        for (int t = 0; t < valid; ++t) {  // slot 4T + i of quarter jj of the lane that holds group g's minima
+          const int n = 4 * (t / 16) + t % 4;
+          uint32_t mine = x.vm[0];
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
-          if ((nan[n] >> lane) & 1) w[n / 2] &= n % 2 ? 0x0000FFFFu : 0xFFFF0000u;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
+          for (int i = 1; i < 4; ++i) mine = n / 2 == i ? x.vm[i] : mine;
+          mine = n % 2 ? mine >> 16 : mine & 0xFFFFu;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            bool hit = false;
-            for (int n = 0; n < 8; ++n)
-              for (int jj = 0; jj < 4; ++jj)
-                hit |= 4 * j + i < F::NG && ((nan[n] >> (16 * jj + 4 * j + i)) & 1) &&
-                       pos + 16 * (n / 4) + 4 * jj + n % 4 <= q.limit[rt];
-            if (hit) st.tail[rt][i] = __builtin_nanf("");
+            const int g = 4 * j + i;
+            const uint32_t h = __shfl(mine, t / 4 % 4 * 16 + g % F::NG);
+            if (g < F::NG && (h & 0x7fffu) > 0x7c00u) {
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt)
+                if (pos + t <= q.limit[rt]) st.tail[rt][i] = __builtin_nanf("");
+            }
           }
         }
       }
@@ -522,26 +564,30 @@ struct Share {
   __device__ inline int64_t owner(int64_t u) const { return ((u + 1) * groups - 1) / units; }
 };
 
-template <int NC>
-struct CombineSmem {
-  static constexpr int kChunk = NC < 8 ? NC : 8;
-  float m[kWaves][16];
-  float l[kWaves][16];
-  float acc[kWaves][kChunk * 4][kWave];
-};
+// The waves' sums meet in the stage, a chunk of channels at a time.
+template <int D>
+constexpr int kChunk = D / 32;
+static_assert(kWaves * kChunk<64> * 4 * kWave * sizeof(float) <= kWaves * Format<64>::kRecord, "a chunk fits a stage");
+static_assert(kWaves * kChunk<128> * 4 * kWave * sizeof(float) <= kWaves * Format<128>::kRecord, "a chunk fits a stage");
+static_assert(kWaves * kChunk<256> * 4 * kWave * sizeof(float) <= kWaves * Format<256>::kRecord, "a chunk fits a stage");
 
-__device__ inline void store_out(const Params& p, int64_t token, int head, int D, int ch, const float* x, int n) {
+template <int N>
+__device__ inline void store_out(const Params& p, int64_t token, int head, int D, int ch, const float (&x)[N]) {
   const int64_t at = (token * p.query_heads + head) * D + ch;
-  if (n == 8) {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = x[i];
-    store8(p.out, at, p.type, v);
+  if constexpr (N == 8) {
+    store8(p.out, at, p.type, x);
   } else if (p.type == kF32) {
-    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(x[0], x[1], x[2], x[3]);
+    float* o = static_cast<float*>(p.out) + at;
+    if constexpr (N == 4)
+      *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
+    else
+      *reinterpret_cast<float2*>(o) = make_float2(x[0], x[1]);
   } else {
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
-        make_uint2(pack2(x[0], x[1], p.type), pack2(x[2], x[3], p.type));
+    uint16_t* o = static_cast<uint16_t*>(p.out) + at;
+    if constexpr (N == 4)
+      *reinterpret_cast<uint2*>(o) = make_uint2(pack2(x[0], x[1], p.type), pack2(x[2], x[3], p.type));
+    else
+      *reinterpret_cast<uint32_t*>(o) = pack2(x[0], x[1], p.type);
   }
 }
 
@@ -552,16 +598,24 @@ struct Target {
   int row0;        // first row of the tile (row = token * group + head)
 };
 
+// Workgroups a compute unit holds, by their registers.
+template <int D, int RT>
+constexpr int kPerCu = D == 256 ? 1 : RT == 1 ? 3 : 2;
+
 template <int D, int RT, bool kFine, bool kCausal>
-__global__ __launch_bounds__(kThreads, RT == 1 && D <= 128 ? 2 : 1) void kv4_attention_kernel(const Params p) {
+__global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kernel(const Params p) {
   using F = Format<D>;
   constexpr int kRows = rows_of(RT);
   constexpr int kRecFloats = static_cast<int>(record_floats(D, kRows));
-  __shared__ CombineSmem<F::NC> cs;
-  __shared__ int64_t s_sum[kThreads + 1];
+  __shared__ __align__(16) uint8_t s_stage[kWaves][F::kRecord];
+  __shared__ float s_m[kWaves][16];
+  __shared__ float s_l[kWaves][16];
   __shared__ int s_last;
+  static_assert(sizeof(s_stage) >= (kThreads + 1) * sizeof(int64_t), "the sums over the lists fit a stage");
+  int64_t* s_sum = reinterpret_cast<int64_t*>(&s_stage[0][0]);
+  float* s_acc = reinterpret_cast<float*>(&s_stage[0][0]);
   const int tid = threadIdx.x;
-  const int wave = tid / kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lane = tid % kWave;
   const int r = lane % 16, j = lane / 16;
   const int64_t w = blockIdx.x;
@@ -622,6 +676,7 @@ __global__ __launch_bounds__(kThreads, RT == 1 && D <= 128 ? 2 : 1) void kv4_att
     }
     s = lo * per;
     base = s_sum[lo];
+    __syncthreads();  // the sums are read: records may be fetched over them
   }
 
   while (u < end) {
@@ -680,14 +735,21 @@ __global__ __launch_bounds__(kThreads, RT == 1 && D <= 128 ? 2 : 1) void kv4_att
       PageRef ref{0, 0};
       if (mine < p1) ref = resolve(p, b, L, mine);
       const int n = min(kWave, (p1 - at + kWaves - 1) / kWaves);
-      for (int k = 0; k < n; ++k) {
-        const int valid = __builtin_amdgcn_readlane(ref.valid, k);
-        if (valid <= 0) continue;
+      const auto fetch = [&](int k) {
         const int64_t page = __builtin_amdgcn_readlane(ref.page, k);
+        fetch_record<D>(p.pool + (page * page_bytes + head_off), s_stage[wave], lane);
+      };
+      fetch(0);
+      for (int k = 0; k < n; ++k) {
+        wait_fetch();
         Record<D> x;
-        load_record<D>(p.pool + page * page_bytes + head_off, lane, x);
-        attend<D, RT, kFine, kCausal>(x, valid, static_cast<int64_t>(at + kWaves * k) * kPageTokens, first_limit, q, st,
-                                      lane);
+        read_record<D>(s_stage[wave], lane, x);
+        wait_reads();
+        if (k + 1 < n) fetch(k + 1);
+        const int valid = __builtin_amdgcn_readlane(ref.valid, k);
+        if (valid > 0)
+          attend<D, RT, kFine, kCausal>(x, valid, static_cast<int64_t>(at + kWaves * k) * kPageTokens, first_limit, q, st,
+                                        lane);
       }
     }
 
@@ -705,47 +767,47 @@ __global__ __launch_bounds__(kThreads, RT == 1 && D <= 128 ? 2 : 1) void kv4_att
 #pragma unroll
         for (int n = 0; n < F::NC; ++n) st.acc[rt][n][i] += add;
       }
-      __syncthreads();  // the last round's readers are done
+      __syncthreads();  // the stages are done with, and the last round's readers
       if (j == 0) {
-        cs.m[wave][r] = st.m[rt];
-        cs.l[wave][r] = l;
+        s_m[wave][r] = st.m[rt];
+        s_l[wave][r] = l;
       }
       __syncthreads();
       float top = kNegInf, sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) top = fmaxf(top, cs.m[i][r]);
+      for (int i = 0; i < kWaves; ++i) top = fmaxf(top, s_m[i][r]);
 #pragma unroll
       for (int i = 0; i < kWaves; ++i)
-        if (cs.m[i][r] != kNegInf || cs.l[i][r] != 0.0f)
-          sum = __builtin_fmaf(cs.l[i][r], cs.m[i][r] == top ? 1.0f : __builtin_amdgcn_exp2f(cs.m[i][r] - top), sum);
+        if (s_m[i][r] != kNegInf || s_l[i][r] != 0.0f)
+          sum = __builtin_fmaf(s_l[i][r], s_m[i][r] == top ? 1.0f : __builtin_amdgcn_exp2f(s_m[i][r] - top), sum);
       const float f = st.m[rt] == top ? 1.0f : __builtin_amdgcn_exp2f(st.m[rt] - top);
       const int row = rt * 16 + r;
       const int token = (tg.row0 + row) / p.group, qh = tg.head0 + (tg.row0 + row) % p.group;
-      constexpr int kChunk = CombineSmem<F::NC>::kChunk;
+      constexpr int kN = kChunk<D>;
 #pragma unroll
-      for (int c = 0; c < F::NC / kChunk; ++c) {
+      for (int c = 0; c < F::NC / kN; ++c) {
         if (c) __syncthreads();
 #pragma unroll
-        for (int n = 0; n < kChunk; ++n)
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) cs.acc[wave][n * 4 + i][lane] = st.acc[rt][c * kChunk + n][i] * f;
+          for (int i = 0; i < 4; ++i) s_acc[((wave * kN + n) * 4 + i) * kWave + lane] = st.acc[rt][c * kN + n][i] * f;
         __syncthreads();
         if (row < live_rows) {  // wave i adds up channels (4j + i) NC ..
-          float x[kChunk];
+          float x[kN];
 #pragma unroll
-          for (int n = 0; n < kChunk; ++n) {
+          for (int n = 0; n < kN; ++n) {
             x[n] = 0.0f;
 #pragma unroll
-            for (int v = 0; v < kWaves; ++v) x[n] += cs.acc[v][n * 4 + wave][lane];
+            for (int v = 0; v < kWaves; ++v) x[n] += s_acc[((v * kN + n) * 4 + wave) * kWave + lane];
           }
-          const int ch = (4 * j + wave) * F::NC + c * kChunk;
+          const int ch = (4 * j + wave) * F::NC + c * kN;
           if (whole) {
 #pragma unroll
-            for (int n = 0; n < kChunk; ++n) x[n] = sum == 0.0f ? 0.0f : x[n] / sum;
-            store_out(p, tg.token0 + token, qh, D, ch, x, kChunk);
+            for (int n = 0; n < kN; ++n) x[n] = sum == 0.0f ? 0.0f : x[n] / sum;
+            store_out(p, tg.token0 + token, qh, D, ch, x);
           } else {
 #pragma unroll
-            for (int n = 0; n < kChunk; ++n) store_agent(rec + 2 * kRows + row * D + ch + n, x[n]);
+            for (int n = 0; n < kN; ++n) store_agent(rec + 2 * kRows + row * D + ch + n, x[n]);
             if (c == 0 && wave == 0 && j == 0) {
               store_agent(rec + 2 * row, top);
               store_agent(rec + 2 * row + 1, sum);
@@ -773,10 +835,11 @@ __global__ __launch_bounds__(kThreads, RT == 1 && D <= 128 ? 2 : 1) void kv4_att
         }
 #pragma unroll
         for (int n = 0; n < 4; ++n) x[n] = sum == 0.0f ? 0.0f : x[n] / sum;
-        store_out(p, tg.token0 + (tg.row0 + row) / p.group, tg.head0 + (tg.row0 + row) % p.group, D, ch, x, 4);
+        store_out(p, tg.token0 + (tg.row0 + row) / p.group, tg.head0 + (tg.row0 + row) % p.group, D, ch, x);
       }
     }
 
+    __syncthreads();  // the next list's records may be fetched over the sums
     u = list_first + p1;
     if constexpr (kCausal) {
       if (p1 == pages && ++s == static_cast<int>(p.tile_info[0])) s = 0;
@@ -876,7 +939,10 @@ __global__ __launch_bounds__(kTileThreads) void tiles_kernel(const Params p, int
 
 // ---- launch ----------------------------------------------------------------------
 
-int grid_groups() { return std::min(kMaxGroups, compute_units() * kGroupsPerCu); }
+int grid_groups(int head_dim, int RT) {
+  const int per_cu = head_dim == 256 ? kPerCu<256, 1> : RT == 1 ? kPerCu<128, 1> : kPerCu<128, 2>;
+  return std::min(kMaxGroups, compute_units() * per_cu);
+}
 
 // Rows of a workgroup's tile: one token a sequence has `group` rows.
 // Two tiles of 16 rows fit the registers up to head_dim 128.
@@ -895,7 +961,7 @@ Layout layout(int64_t batch, int64_t tokens, int group, int head_dim, int RT) {
   const size_t counters = kMaxGroups * sizeof(int32_t);
   const int64_t tiles = max_tiles(batch, tokens, group, rows_of(RT));
   l.records = counters;
-  l.info = l.records + 2 * static_cast<size_t>(grid_groups()) * record_floats(head_dim, rows_of(RT)) * sizeof(float);
+  l.info = l.records + 2 * static_cast<size_t>(grid_groups(head_dim, RT)) * record_floats(head_dim, rows_of(RT)) * sizeof(float);
   l.info = (l.info + 255) / 256 * 256;
   l.first = l.info + 256;
   l.tiles = (l.first + tiles * sizeof(int64_t) + 255) / 256 * 256;
@@ -905,7 +971,7 @@ Layout layout(int64_t batch, int64_t tokens, int group, int head_dim, int RT) {
 
 template <int D, int RT, bool kCausal>
 void launch_typed(const Params& p, bool fine, hipStream_t stream) {
-  const dim3 grid(grid_groups());
+  const dim3 grid(grid_groups(D, RT));
   if (fine)
     hipLaunchKernelGGL((kv4_attention_kernel<D, RT, true, kCausal>), grid, dim3(kThreads), 0, stream, p);
   else

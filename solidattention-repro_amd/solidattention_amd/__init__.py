@@ -815,59 +815,78 @@ POOL_KV4 = 0x4B563434
 F32, F16, BF16 = 0, 1, 2
 
 
+def _torch():
+    global _torch_module, _TYPES, _INT32
+    import torch
+    _torch_module = torch
+    _TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    _INT32 = torch.int32
+    return torch
+
+
+_torch_module = None
+_TYPES: dict = {}
+_INT32 = None
+
+
 class _On:
     """The device of a call's tensors made current, and the stream that the call runs on (the given one, or that
-    device's current one); what is allocated inside belongs to that stream."""
+    device's current one); what is allocated inside belongs to that stream.  Where both are current already there is
+    nothing to switch."""
+    __slots__ = ("device", "stream", "scopes")
 
     def __init__(self, device, stream=None):
-        import torch
-        self.device = torch.cuda.device(device)
-        self.given = stream
-        self.place = device
+        self.device, self.stream, self.scopes = device, stream, ()
 
     def __enter__(self):
-        import torch
-        self.device.__enter__()
-        s = self.given if self.given is not None else torch.cuda.current_stream(self.place)
-        self.scope = torch.cuda.stream(s)
-        self.scope.__enter__()
-        return C.c_void_p(s.cuda_stream)
+        cuda = (_torch_module or _torch()).cuda
+        s = self.stream
+        if s is not None or self.device.index != cuda.current_device():
+            self.scopes = (cuda.device(self.device), cuda.stream(s))  # (a stream of None leaves the stream)
+            for scope in self.scopes:
+                scope.__enter__()
+        if s is None:
+            s = cuda.current_stream(self.device)
+        return s.cuda_stream
 
     def __exit__(self, *a):
-        self.scope.__exit__(*a)
-        return self.device.__exit__(*a)
+        for scope in reversed(self.scopes):
+            scope.__exit__(*a)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _type_of(x, what):
-    import torch
-    types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    if x.dtype not in types:
+    type_ = _TYPES.get(x.dtype)
+    if type_ is None:
         raise ValueError(f"{what}: {x.dtype} is not float32, float16 or bfloat16")
-    return types[x.dtype]
+    return type_
 
 
 def _heads_rows(x, heads, head_dim, what, device):
     """Elements between the tokens of x [tokens][heads][head_dim], whose rows are whole."""
-    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != head_dim:
-        raise ValueError(f"{what}: shape {tuple(x.shape)} is not [tokens, {heads}, {head_dim}]")
+    shape, row = x.shape, heads * head_dim
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
+        raise ValueError(f"{what}: shape {tuple(shape)} is not [tokens, {heads}, {head_dim}]")
     if x.device != device:
         raise ValueError(f"{what} is on {x.device}, the cache on {device}")
-    if x.stride(2) != 1 or (heads > 1 and x.stride(1) != head_dim):
+    s0, s1, s2 = x.stride()
+    if s2 != 1 or (heads > 1 and s1 != head_dim):
         raise ValueError(f"{what}: a token's heads must be contiguous (strides {x.stride()})")
-    if x.shape[0] <= 1:
-        return heads * head_dim
-    if x.stride(0) < heads * head_dim:
+    if shape[0] <= 1:
+        return row
+    if s0 < row:
         raise ValueError(f"{what}: rows overlap (strides {x.stride()})")
-    return x.stride(0)
+    return s0
 
 
 def _ints(x, count, what, device):
-    import torch
-    if x.dtype != torch.int32 or not x.is_contiguous() or x.numel() < count:
+    if x.dtype != (_INT32 or _torch().int32) or x.numel() < count or not x.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of at least {count} elements")
     if x.device != device:
         raise ValueError(f"{what} is on {x.device}, the cache on {device}")
-    return x
 
 
 class PagedKV4(PagedKV):
@@ -893,9 +912,11 @@ class PagedKV4(PagedKV):
                          rep_stride=rep_stride, head_dim=head_dim, device=pool.device, pool=pool)
 
     def struct(self) -> PagedKVStruct:
-        s = super().struct()
-        s.reserved = POOL_KV4
-        return s
+        return PagedKVStruct(
+            self.pool.data_ptr(), self.block_table.data_ptr(), self.seq_len.data_ptr(),
+            self.sealed.data_ptr(), self.generation.data_ptr(), self.reps.data_ptr(),
+            self.num_pages, self.batch, self.table_stride, self.rep_heads, self.rep_stride,
+            self.query_heads, self.kv_heads, self.head_dim, POOL_KV4)
 
     @property
     def page_bytes(self) -> int:
@@ -922,9 +943,9 @@ def reserve_tokens(kv: PagedKV, new_tokens, free_pages, free_count, query_start,
         _ints(positions, slots.numel(), "positions", dev)
     s = kv.struct()
     with _On(dev, stream) as st:
-        check(lib().sa_hip_reserve_tokens(C.byref(s), _ptr(new_tokens), _ptr(free_pages), _ptr(free_count),
-                                          slots.numel(), _ptr(query_start), _ptr(slots), _ptr(positions),
-                                          _ptr(seq_len_out), _ptr(free_count_out), _ptr(status), st),
+        check(lib().sa_hip_reserve_tokens(C.byref(s), _addr(new_tokens), _addr(free_pages), _addr(free_count),
+                                          slots.numel(), _addr(query_start), _addr(slots), _addr(positions),
+                                          _addr(seq_len_out), _addr(free_count_out), _addr(status), st),
               "reserve_tokens")
     return query_start, slots, positions
 
@@ -944,12 +965,14 @@ def release_sequences(kv: PagedKV, finished, free_pages, free_count, seq_len_out
         _ints(x, n, what, dev)
     s = kv.struct()
     with _On(dev, stream) as st:
-        check(lib().sa_hip_release_sequences(C.byref(s), _ptr(finished), _ptr(free_pages), _ptr(free_count),
-                                             _ptr(seq_len_out), _ptr(free_count_out), _ptr(status), st),
+        check(lib().sa_hip_release_sequences(C.byref(s), _addr(finished), _addr(free_pages), _addr(free_count),
+                                             _addr(seq_len_out), _addr(free_count_out), _addr(status), st),
               "release_sequences")
 
 
 def _kv4_rows(kv, k, v, tokens):
+    if _torch_module is None:
+        _torch()
     dev = kv.pool.device
     stride = [_heads_rows(x, kv.kv_heads, kv.head_dim, what, dev) for x, what in ((k, "k"), (v, "v"))]
     if k.dtype != v.dtype or k.shape[0] != v.shape[0] or k.shape[0] < tokens:
@@ -965,7 +988,7 @@ def kv4_store(kv: PagedKV4, k, v, slots, status=None, stream=None):
     _ints(slots, n, "slots", kv.pool.device)
     s = kv.struct()
     with _On(kv.pool.device, stream) as st:
-        check(lib().sa_hip_kv4_store(C.byref(s), _ptr(k), _ptr(v), type_, ks, vs, _ptr(slots), n, _ptr(status), st),
+        check(lib().sa_hip_kv4_store(C.byref(s), _addr(k), _addr(v), type_, ks, vs, _addr(slots), n, _addr(status), st),
               "kv4_store")
 
 
@@ -976,7 +999,7 @@ def kv4_load(kv: PagedKV4, slots, k, v, status=None, stream=None):
     _ints(slots, n, "slots", kv.pool.device)
     s = kv.struct()
     with _On(kv.pool.device, stream) as st:
-        check(lib().sa_hip_kv4_load(C.byref(s), _ptr(k), _ptr(v), type_, ks, vs, _ptr(slots), n, _ptr(status), st),
+        check(lib().sa_hip_kv4_load(C.byref(s), _addr(k), _addr(v), type_, ks, vs, _addr(slots), n, _addr(status), st),
               "kv4_load")
     return k, v
 
@@ -986,7 +1009,7 @@ def kv4_append_seal(kv: PagedKV4, k, v, local_tokens, status=None, stream=None):
     type_, ks, vs = _kv4_rows(kv, k, v, kv.batch)
     s = kv.struct()
     with _On(kv.pool.device, stream) as st:
-        check(lib().sa_hip_kv4_append_seal(C.byref(s), _ptr(k), _ptr(v), type_, ks, vs, local_tokens, _ptr(status),
+        check(lib().sa_hip_kv4_append_seal(C.byref(s), _addr(k), _addr(v), type_, ks, vs, local_tokens, _addr(status),
                                            st), "kv4_append_seal")
 
 
@@ -994,7 +1017,7 @@ def kv4_seal(kv: PagedKV4, local_tokens, status=None, stream=None):
     """seal on 4-bit pages (after kv4_store wrote a prompt and its lengths were set)."""
     s = kv.struct()
     with _On(kv.pool.device, stream) as st:
-        check(lib().sa_hip_kv4_seal(C.byref(s), local_tokens, _ptr(status), st), "kv4_seal")
+        check(lib().sa_hip_kv4_seal(C.byref(s), local_tokens, _addr(status), st), "kv4_seal")
 
 
 def kv4_attention_workspace(kv: PagedKV4, query_tokens=None):
@@ -1006,18 +1029,26 @@ def kv4_attention_workspace(kv: PagedKV4, query_tokens=None):
     return torch.zeros(max(n, 16), dtype=torch.uint8, device=kv.pool.device)
 
 
-def _kv4_attention(kv, query, out, workspace):
-    import torch
+def _kv4_query(kv, query, out, workspace):
+    """Elements between the query's tokens; out and workspace, where given, fit it."""
+    if _torch_module is None:
+        _torch()
     stride = _heads_rows(query, kv.query_heads, kv.head_dim, "query", kv.pool.device)
-    if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    elif out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous() or out.device != query.device:
+    _type_of(query, "query")
+    if out is not None and (out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous() or
+                            out.device != query.device):
         raise ValueError("out must be contiguous, of the query's shape, dtype and device")
+    if workspace is not None and (workspace.device != query.device or not workspace.is_contiguous()):
+        raise ValueError("workspace must be contiguous and on the query's device")
+    return stride
+
+
+def _kv4_buffers(kv, query, out, workspace):
+    if out is None:
+        out = _torch_module.empty(query.shape, dtype=query.dtype, device=query.device)
     if workspace is None:
         workspace = kv4_attention_workspace(kv, query.shape[0])
-    elif workspace.device != query.device or not workspace.is_contiguous():
-        raise ValueError("workspace must be contiguous and on the query's device")
-    return stride, out, workspace, workspace.numel() * workspace.element_size()
+    return out, workspace, workspace.numel() * workspace.element_size()
 
 
 def kv4_decode_attention(kv: PagedKV4, query, scale, selected=None, counts=None, out=None, workspace=None,
@@ -1032,12 +1063,13 @@ def kv4_decode_attention(kv: PagedKV4, query, scale, selected=None, counts=None,
         groups, sel_stride = selected.shape[1], selected.shape[2]
         _ints(selected, kv.batch * groups * sel_stride, "selected", kv.pool.device)
         _ints(counts, kv.batch * groups, "counts", kv.pool.device)
+    stride = _kv4_query(kv, query, out, workspace)
     s = kv.struct()
     with _On(kv.pool.device, stream) as st:
-        stride, out, workspace, nbytes = _kv4_attention(kv, query, out, workspace)
+        out, workspace, nbytes = _kv4_buffers(kv, query, out, workspace)
         check(lib().sa_hip_kv4_decode_attention(
-            C.byref(s), _ptr(query), _type_of(query, "query"), stride, _ptr(selected), _ptr(counts), groups,
-            sel_stride, C.c_float(scale), _ptr(out), _ptr(workspace), nbytes, _ptr(status), st),
+            C.byref(s), _addr(query), _type_of(query, "query"), stride, _addr(selected), _addr(counts), groups,
+            sel_stride, scale, _addr(out), _addr(workspace), nbytes, _addr(status), st),
             "kv4_decode_attention")
     return out
 
@@ -1047,12 +1079,13 @@ def kv4_prompt_attention(kv: PagedKV4, query, query_start, scale, out=None, work
     [query_start[b], query_start[b + 1]) of query [tokens, query_heads, head_dim] are the last tokens of sequence b.
     Rows outside every range are left as they are."""
     _ints(query_start, kv.batch + 1, "query_start", kv.pool.device)
+    stride = _kv4_query(kv, query, out, workspace)
     s = kv.struct()
     with _On(kv.pool.device, stream) as st:
-        stride, out, workspace, nbytes = _kv4_attention(kv, query, out, workspace)
+        out, workspace, nbytes = _kv4_buffers(kv, query, out, workspace)
         check(lib().sa_hip_kv4_prompt_attention(
-            C.byref(s), _ptr(query), _type_of(query, "query"), stride, _ptr(query_start), query.shape[0],
-            C.c_float(scale), _ptr(out), _ptr(workspace), nbytes, _ptr(status), st), "kv4_prompt_attention")
+            C.byref(s), _addr(query), _type_of(query, "query"), stride, _addr(query_start), query.shape[0],
+            scale, _addr(out), _addr(workspace), nbytes, _addr(status), st), "kv4_prompt_attention")
     return out
 
 
