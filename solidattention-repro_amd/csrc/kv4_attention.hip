@@ -24,8 +24,7 @@
 // lists form one row of units, and each workgroup takes an equal share of it,
 // whatever the lists' lengths.  A list cut by a share's border is merged by the
 // last workgroup to finish it.
-#include "kv4_format.hpp"
-#include "sa_internal.hpp"
+#include "kv4_attention.hpp"
 
 #include <algorithm>
 
@@ -34,19 +33,8 @@ namespace {
 
 using namespace kv4;
 
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kMaxGroups = 4096;   // workgroups, and arrival counters at the front of the workspace
-constexpr int kMinUnits = 8;       // pages a workgroup is worth starting for
-constexpr float kNegInf = -__builtin_huge_valf();
-constexpr float kLowest = -3.0e38f;  // of masked scores: finite, so that a factor of 0 leaves no NaN
-constexpr float kLog2e = 1.4426950408889634f;
-
 // Probabilities are held times 2^shift, against a maximum that may lag the
 // true one by `lag` (in exponents of 2): they stay below FP16's largest
 // number, and down to 2^-(25 + shift) of the row's largest they are not lost.
@@ -55,107 +43,6 @@ template <bool kFine>
 constexpr float kShift = kFine ? 14.0f : 6.0f;
 template <bool kFine>
 constexpr float kLag = kFine ? 1.0f : 9.0f;
-
-struct Params {
-  const uint8_t* pool;
-  const int32_t* table;
-  const int32_t* seq_len;
-  const int32_t* sealed;
-  const int32_t* selected;
-  const int32_t* counts;
-  const int32_t* query_start;
-  const void* query;
-  void* out;
-  int32_t* status;
-  int32_t* arrive;
-  float* records;
-  int64_t* tile_info;  // prompt: [0] tiles, [1] units of one KV head
-  int64_t* tile_first; // units before a tile
-  int4* tiles;         // (sequence, first row, pages, -)
-  int64_t num_pages;
-  int64_t q_stride;
-  int32_t tokens;
-  int32_t batch;
-  int32_t table_stride;
-  int32_t sel_stride;
-  int32_t select_groups;
-  int32_t kv_per_sel;
-  int32_t query_heads;
-  int32_t kv_heads;
-  int32_t group;
-  int32_t type;
-  float qscale;
-};
-
-// ---- lists of pages -----------------------------------------------------------
-
-struct List {
-  const int32_t* sel;
-  int64_t len;   // tokens that may be read
-  int sealed;    // blocks the list's tail starts behind
-  int n_sel;
-  int total;     // pages
-};
-
-// One token a sequence: the selected blocks then the tail, or every page.
-// Inconsistent lengths are flagged and clamped to what can be read safely.
-__device__ inline List decode_list(const Params& p, int b, int sg) {
-  List L{nullptr, p.seq_len[b], 0, 0, 0};
-  bool bad = L.len < 0;
-  if (p.selected) {
-    L.sealed = p.sealed[b];
-    L.n_sel = p.counts[static_cast<int64_t>(b) * p.select_groups + sg];
-    L.sel = p.selected + (static_cast<int64_t>(b) * p.select_groups + sg) * p.sel_stride;
-    bad = bad || L.sealed < 0 || L.len < static_cast<int64_t>(L.sealed) * kPageTokens;
-    if (L.n_sel < 0 || L.n_sel > p.sel_stride) {
-      L.n_sel = 0;
-      flag_status(p.status, kStatusBadLength);
-    }
-  }
-  if (bad) {
-    flag_status(p.status, kStatusBadLength);
-    if (L.sealed < 0) L.sealed = 0;
-    L.len = static_cast<int64_t>(L.sealed) * kPageTokens;
-  }
-  const int64_t tail = L.len - static_cast<int64_t>(L.sealed) * kPageTokens;
-  L.total = L.n_sel + static_cast<int>((tail + kPageTokens - 1) / kPageTokens);
-  return L;
-}
-
-struct PageRef {
-  int32_t page;   // a readable page in any case
-  int32_t valid;  // its tokens (0: skip)
-};
-
-__device__ inline PageRef resolve(const Params& p, int b, const List& L, int i) {
-  PageRef r{0, 0};
-  if (i >= L.total) return r;
-  int64_t logical;
-  int valid = kPageTokens;
-  if (i < L.n_sel) {
-    logical = L.sel[i];
-    if (logical < 0 || logical >= L.sealed) {
-      flag_status(p.status, kStatusBadBlock);
-      return r;
-    }
-  } else {
-    logical = static_cast<int64_t>(L.sealed) + (i - L.n_sel);
-    const int64_t left = L.len - logical * kPageTokens;
-    if (left < kPageTokens) valid = static_cast<int>(left);
-  }
-  if (logical >= p.table_stride) {
-    flag_status(p.status, kStatusBadBlock);
-    return r;
-  }
-  const int32_t page = p.table[static_cast<int64_t>(b) * p.table_stride + logical];
-  if (page < 0 || page >= p.num_pages) {
-    flag_status(p.status, kStatusBadPage);
-    return r;
-  }
-  r.page = page;
-  r.valid = valid;
-  return r;
-}
 
 // ---- a record in LDS -------------------------------------------------------------
 // A wave copies its next record from memory straight into its LDS slot while it
@@ -220,42 +107,6 @@ __device__ inline void read_record(const uint8_t* slot, int lane, Record<D>& x) 
   read_words<4>(slot + F::kValueScales + (r * F::NC / 32 * 4 + j) * 16, x.vs);
 }
 
-__device__ inline half8 as_half8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return __builtin_bit_cast(half8, u32x4{a, b, c, d});
-}
-__device__ inline half2_t as_half2(uint32_t a) { return __builtin_bit_cast(half2_t, a); }
-__device__ inline uint32_t bits_of(half2_t a) { return __builtin_bit_cast(uint32_t, a); }
-
-// x & mask | base in one instruction (the compiler splits it over two literals).
-__device__ inline uint32_t and_or(uint32_t x, uint32_t mask, uint32_t base) {
-  uint32_t d;
-  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(d) : "v"(x), "s"(mask), "v"(base));
-  return d;
-}
-
-// Nibbles 0 and 1 of both halves as FP16 integers: moved into the mantissa of
-// 1024.0 (bits 0..3) or 64.0 (bits 4..7), which is then taken off (exact).
-__device__ inline half2_t low_nibbles(uint32_t w) { return as_half2(and_or(w, 0x000F000Fu, 0x64006400u)) - half2_t{1024, 1024}; }
-__device__ inline half2_t high_nibbles(uint32_t w) { return as_half2(and_or(w, 0x00F000F0u, 0x54005400u)) - half2_t{64, 64}; }
-
-// 8 nibbles in the order (0,4), (1,5), (2,6), (3,7).
-__device__ inline half8 key_codes(uint32_t w) {
-  return as_half8(bits_of(low_nibbles(w)), bits_of(high_nibbles(w)), bits_of(low_nibbles(w >> 8)),
-                  bits_of(high_nibbles(w >> 8)));
-}
-
-// Nibble n (0..3) of both halves as FP16 integers times the pair of scales
-// (exact: 4 + 7 bits).
-template <int N>
-__device__ inline uint32_t scaled_codes(uint32_t y, uint32_t scales) {
-  const uint32_t w = N < 2 ? y : y >> 8;
-  return bits_of((N % 2 == 0 ? low_nibbles(w) : high_nibbles(w)) * as_half2(scales));
-}
-
-__device__ inline f32x4 mfma(half8 a, half8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
 // The value operand of channel n of every row: slots 8j.. of tiles 0 and 1.
 template <int D, int N>
 __device__ inline half8 value_operand(const Record<D>& x) {
@@ -292,8 +143,6 @@ struct Rows {
   float factor[RT];
   int64_t limit[RT];      // last position the row sees
 };
-
-__device__ inline float ldexp2(float x, int e) { return __builtin_ldexpf(x, e); }
 
 template <int D, int RT, bool kFine>
 __device__ inline void load_rows(const Params& p, Rows<D, RT, kFine>& q, int64_t token0, int n_tokens, int head0,
@@ -557,13 +406,6 @@ __device__ inline float tile_row(const f32x4& t, int row, int lane) {
 constexpr int rows_of(int RT) { return 16 * RT; }
 constexpr size_t record_floats(int D, int rows) { return static_cast<size_t>(rows) * (D + 2); }
 
-struct Share {
-  int64_t units;   // of the whole launch
-  int64_t groups;  // workgroups that take part
-  __device__ inline int64_t begin(int64_t w) const { return units * w / groups; }
-  __device__ inline int64_t owner(int64_t u) const { return ((u + 1) * groups - 1) / units; }
-};
-
 // The waves' sums meet in the stage, a chunk of channels at a time.
 template <int D>
 constexpr int kChunk = D / 32;
@@ -590,13 +432,6 @@ __device__ inline void store_out(const Params& p, int64_t token, int head, int D
       *reinterpret_cast<uint32_t*>(o) = pack2(x[0], x[1], p.type);
   }
 }
-
-struct Target {
-  int64_t token0;  // first query row of the sequence
-  int n_tokens;
-  int head0;       // first query head
-  int row0;        // first row of the tile (row = token * group + head)
-};
 
 // Workgroups a compute unit holds, by their registers.
 template <int D, int RT>
@@ -944,25 +779,37 @@ int grid_groups(int head_dim, int RT) {
   return std::min(kMaxGroups, compute_units() * per_cu);
 }
 
-// Rows of a workgroup's tile: one token a sequence has `group` rows.
-// Two tiles of 16 rows fit the registers up to head_dim 128.
-int row_tiles(bool prompt, int head_dim) { return prompt && head_dim <= 128 ? 2 : 1; }
+// How a call runs: one token a sequence in a tile of 16 rows; several in this
+// file's tiles of 32 rows (16 at head_dim 256, by the registers), or in
+// kv4_prompt.hip's of many.
+enum class Form { kDecode, kFew, kMany };
 
-int64_t max_tiles(int64_t batch, int64_t tokens, int group, int rows) {
-  return tokens * group / rows + std::min(batch, tokens) + 1;
+struct Plan {
+  int rows;         // of a tile
+  size_t records;   // bytes
+};
+
+Plan plan(Form form, int head_dim) {
+  if (form == Form::kMany)
+    return {prompt_tile_rows(head_dim), 2 * prompt_groups(head_dim) * prompt_record_floats(head_dim) * sizeof(float)};
+  const int RT = form == Form::kFew && head_dim <= 128 ? 2 : 1;
+  return {rows_of(RT), 2 * grid_groups(head_dim, RT) * record_floats(head_dim, rows_of(RT)) * sizeof(float)};
+}
+
+Form form_of(bool prompt, int64_t tokens, int64_t batch, int group, int type) {
+  if (!prompt) return Form::kDecode;
+  return type != kF32 && tokens * group >= 64 * batch ? Form::kMany : Form::kFew;
 }
 
 struct Layout {
   size_t records, info, first, tiles, bytes;
 };
 
-Layout layout(int64_t batch, int64_t tokens, int group, int head_dim, int RT) {
+Layout layout(const Plan& pl, int64_t batch, int64_t tokens, int group) {
   Layout l{};
-  const size_t counters = kMaxGroups * sizeof(int32_t);
-  const int64_t tiles = max_tiles(batch, tokens, group, rows_of(RT));
-  l.records = counters;
-  l.info = l.records + 2 * static_cast<size_t>(grid_groups(head_dim, RT)) * record_floats(head_dim, rows_of(RT)) * sizeof(float);
-  l.info = (l.info + 255) / 256 * 256;
+  const int64_t tiles = max_tiles(batch, tokens, group, pl.rows);
+  l.records = kMaxGroups * sizeof(int32_t);  // behind the arrival counters
+  l.info = (l.records + pl.records + 255) / 256 * 256;
   l.first = l.info + 256;
   l.tiles = (l.first + tiles * sizeof(int64_t) + 255) / 256 * 256;
   l.bytes = l.tiles + tiles * sizeof(int4);
@@ -988,11 +835,24 @@ void launch_dim(const Params& p, bool fine, hipStream_t stream) {
 
 }  // namespace
 
+namespace kv4 {
+
+int64_t max_tiles(int64_t batch, int64_t tokens, int group, int rows) {
+  return tokens * group / rows + std::min(batch, tokens) + 1;
+}
+
+hipError_t launch_tiles(const Params& p, int rows, hipStream_t stream) {
+  hipLaunchKernelGGL(tiles_kernel, dim3(1), dim3(kTileThreads), 0, stream, p, rows);
+  return hipGetLastError();
+}
+
+}  // namespace kv4
+
 size_t kv4_attention_workspace_bytes(int32_t batch, int32_t query_heads, int32_t kv_heads, int32_t head_dim,
                                      int64_t tokens) {
-  size_t bytes = 0;  // either call's
-  for (int RT = 1; RT <= 2; ++RT)
-    bytes = std::max(bytes, layout(batch, tokens, query_heads / kv_heads, head_dim, RT).bytes);
+  size_t bytes = 0;  // any form's
+  for (const Form f : {Form::kDecode, Form::kFew, Form::kMany})
+    bytes = std::max(bytes, layout(plan(f, head_dim), batch, tokens, query_heads / kv_heads).bytes);
   return bytes;
 }
 
@@ -1021,8 +881,9 @@ hipError_t launch_kv4_attention(const Kv4AttnLaunch& a, hipStream_t stream) {
   p.group = a.query_heads / a.kv_heads;
   p.type = a.type;
   p.qscale = a.scale * kLog2e;
-  const int RT = row_tiles(a.query_start != nullptr, a.head_dim);
-  const Layout l = layout(a.batch, a.tokens, p.group, a.head_dim, RT);
+  const Form form = form_of(a.query_start != nullptr, a.tokens, a.batch, p.group, a.type);
+  const Plan pl = plan(form, a.head_dim);
+  const Layout l = layout(pl, a.batch, a.tokens, p.group);
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.arrive = reinterpret_cast<int32_t*>(ws);
   p.records = reinterpret_cast<float*>(ws + l.records);
@@ -1030,10 +891,10 @@ hipError_t launch_kv4_attention(const Kv4AttnLaunch& a, hipStream_t stream) {
   p.tile_first = reinterpret_cast<int64_t*>(ws + l.first);
   p.tiles = reinterpret_cast<int4*>(ws + l.tiles);
   if (a.query_start) {
-    hipLaunchKernelGGL(tiles_kernel, dim3(1), dim3(kTileThreads), 0, stream, p, rows_of(RT));
-    const hipError_t e = hipGetLastError();
+    const hipError_t e = launch_tiles(p, pl.rows, stream);
     if (e != hipSuccess) return e;
   }
+  if (form == Form::kMany) return launch_prompt_tiles(p, a.head_dim, stream);
   const bool fine = a.type == kF32;
   if (a.head_dim == 64) launch_dim<64>(p, fine, stream);
   if (a.head_dim == 128) launch_dim<128>(p, fine, stream);

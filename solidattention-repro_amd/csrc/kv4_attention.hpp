@@ -1,0 +1,197 @@
+// kv4_attention.hpp — what the attention kernels over 4-bit pages share: their
+// parameters, the lists of pages, the operands of the matrix cores, and the
+// split of a launch's pages into equal shares.
+#pragma once
+
+#include "kv4_format.hpp"
+#include "sa_internal.hpp"
+
+namespace sa {
+namespace kv4 {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kMaxGroups = 4096;   // workgroups, and arrival counters at the front of the workspace
+constexpr int kMinUnits = 8;       // pages a workgroup is worth starting for
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLowest = -3.0e38f;  // of masked scores: finite, so that a factor of 0 leaves no NaN
+constexpr float kLog2e = 1.4426950408889634f;
+
+
+struct Params {
+  const uint8_t* pool;
+  const int32_t* table;
+  const int32_t* seq_len;
+  const int32_t* sealed;
+  const int32_t* selected;
+  const int32_t* counts;
+  const int32_t* query_start;
+  const void* query;
+  void* out;
+  int32_t* status;
+  int32_t* arrive;
+  float* records;
+  int64_t* tile_info;  // prompt: [0] tiles, [1] units of one KV head
+  int64_t* tile_first; // units before a tile
+  int4* tiles;         // (sequence, first row, pages, -)
+  int64_t num_pages;
+  int64_t q_stride;
+  int32_t tokens;
+  int32_t batch;
+  int32_t table_stride;
+  int32_t sel_stride;
+  int32_t select_groups;
+  int32_t kv_per_sel;
+  int32_t query_heads;
+  int32_t kv_heads;
+  int32_t group;
+  int32_t type;
+  float qscale;
+};
+
+// ---- lists of pages -----------------------------------------------------------
+
+struct List {
+  const int32_t* sel;
+  int64_t len;   // tokens that may be read
+  int sealed;    // blocks the list's tail starts behind
+  int n_sel;
+  int total;     // pages
+};
+
+// One token a sequence: the selected blocks then the tail, or every page.
+// Inconsistent lengths are flagged and clamped to what can be read safely.
+__device__ inline List decode_list(const Params& p, int b, int sg) {
+  List L{nullptr, p.seq_len[b], 0, 0, 0};
+  bool bad = L.len < 0;
+  if (p.selected) {
+    L.sealed = p.sealed[b];
+    L.n_sel = p.counts[static_cast<int64_t>(b) * p.select_groups + sg];
+    L.sel = p.selected + (static_cast<int64_t>(b) * p.select_groups + sg) * p.sel_stride;
+    bad = bad || L.sealed < 0 || L.len < static_cast<int64_t>(L.sealed) * kPageTokens;
+    if (L.n_sel < 0 || L.n_sel > p.sel_stride) {
+      L.n_sel = 0;
+      flag_status(p.status, kStatusBadLength);
+    }
+  }
+  if (bad) {
+    flag_status(p.status, kStatusBadLength);
+    if (L.sealed < 0) L.sealed = 0;
+    L.len = static_cast<int64_t>(L.sealed) * kPageTokens;
+  }
+  const int64_t tail = L.len - static_cast<int64_t>(L.sealed) * kPageTokens;
+  L.total = L.n_sel + static_cast<int>((tail + kPageTokens - 1) / kPageTokens);
+  return L;
+}
+
+struct PageRef {
+  int32_t page;   // a readable page in any case
+  int32_t valid;  // its tokens (0: skip)
+};
+
+__device__ inline PageRef resolve(const Params& p, int b, const List& L, int i) {
+  PageRef r{0, 0};
+  if (i >= L.total) return r;
+  int64_t logical;
+  int valid = kPageTokens;
+  if (i < L.n_sel) {
+    logical = L.sel[i];
+    if (logical < 0 || logical >= L.sealed) {
+      flag_status(p.status, kStatusBadBlock);
+      return r;
+    }
+  } else {
+    logical = static_cast<int64_t>(L.sealed) + (i - L.n_sel);
+    const int64_t left = L.len - logical * kPageTokens;
+    if (left < kPageTokens) valid = static_cast<int>(left);
+  }
+  if (logical >= p.table_stride) {
+    flag_status(p.status, kStatusBadBlock);
+    return r;
+  }
+  const int32_t page = p.table[static_cast<int64_t>(b) * p.table_stride + logical];
+  if (page < 0 || page >= p.num_pages) {
+    flag_status(p.status, kStatusBadPage);
+    return r;
+  }
+  r.page = page;
+  r.valid = valid;
+  return r;
+}
+
+// ---- operands of the matrix cores ----------------------------------------------
+
+__device__ inline half8 as_half8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(half8, u32x4{a, b, c, d});
+}
+__device__ inline half2_t as_half2(uint32_t a) { return __builtin_bit_cast(half2_t, a); }
+__device__ inline uint32_t bits_of(half2_t a) { return __builtin_bit_cast(uint32_t, a); }
+
+// x & mask | base in one instruction (the compiler splits it over two literals).
+__device__ inline uint32_t and_or(uint32_t x, uint32_t mask, uint32_t base) {
+  uint32_t d;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(d) : "v"(x), "s"(mask), "v"(base));
+  return d;
+}
+
+// Nibbles 0 and 1 of both halves as FP16 integers: moved into the mantissa of
+// 1024.0 (bits 0..3) or 64.0 (bits 4..7), which is then taken off (exact).
+__device__ inline half2_t low_nibbles(uint32_t w) { return as_half2(and_or(w, 0x000F000Fu, 0x64006400u)) - half2_t{1024, 1024}; }
+__device__ inline half2_t high_nibbles(uint32_t w) { return as_half2(and_or(w, 0x00F000F0u, 0x54005400u)) - half2_t{64, 64}; }
+
+// 8 nibbles in the order (0,4), (1,5), (2,6), (3,7).
+__device__ inline half8 key_codes(uint32_t w) {
+  return as_half8(bits_of(low_nibbles(w)), bits_of(high_nibbles(w)), bits_of(low_nibbles(w >> 8)),
+                  bits_of(high_nibbles(w >> 8)));
+}
+
+// Nibble n (0..3) of both halves as FP16 integers times the pair of scales
+// (exact: 4 + 7 bits).
+template <int N>
+__device__ inline uint32_t scaled_codes(uint32_t y, uint32_t scales) {
+  const uint32_t w = N < 2 ? y : y >> 8;
+  return bits_of((N % 2 == 0 ? low_nibbles(w) : high_nibbles(w)) * as_half2(scales));
+}
+
+__device__ inline f32x4 mfma(half8 a, half8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+__device__ inline float ldexp2(float x, int e) { return __builtin_ldexpf(x, e); }
+
+// ---- shares of the row of units ---------------------------------------------------
+// The pages of all lists form one row of units; workgroup w of `groups` takes
+// units [begin(w), begin(w + 1)), whatever lists they belong to.
+
+struct Share {
+  int64_t units;   // of the whole launch
+  int64_t groups;  // workgroups that take part
+  __device__ inline int64_t begin(int64_t w) const { return units * w / groups; }
+  __device__ inline int64_t owner(int64_t u) const { return ((u + 1) * groups - 1) / units; }
+};
+
+struct Target {
+  int64_t token0;  // first query row of the sequence
+  int n_tokens;
+  int head0;       // first query head
+  int row0;        // first row of the tile (row = token * group + head)
+};
+
+// The tiles of `rows` rows each of a batch of query tokens (kv4_attention.hip)
+// into p.tiles, p.tile_first and p.tile_info.
+hipError_t launch_tiles(const Params& p, int rows, hipStream_t stream);
+int64_t max_tiles(int64_t batch, int64_t tokens, int group, int rows);
+
+// Tiles of many rows (kv4_prompt.hip): rows of a tile, workgroups of a launch,
+// floats of one of its two records a workgroup.
+int prompt_tile_rows(int head_dim);
+int prompt_groups(int head_dim);
+size_t prompt_record_floats(int head_dim);
+hipError_t launch_prompt_tiles(const Params& p, int head_dim, hipStream_t stream);
+
+}  // namespace kv4
+}  // namespace sa

@@ -1,0 +1,471 @@
+// kv4_prompt.hip — causal attention of many query rows over the pages held in
+// 4 bits, for 16-bit queries (gfx950).
+//
+// The same sums as kv4_attention.hip, arranged for arithmetic: a workgroup's
+// tile is 256 rows (row = token * group + head) of one KV head, 32 for each of
+// its 8 waves, and all of them attend the same page.  The page's 8 KB of codes
+// are turned into FP16 once, scale * code + minimum rounded once (2^-11
+// relative, as an FP16 cache's own values), by all waves together, into LDS in
+// the order of the operands of v_mfma_f32_32x32x16_f16:
+//   scores   rows = tokens, columns = query rows: lane (column c = lane % 32,
+//            half h = lane / 32) holds tokens 8 (i / 4) + 4 h + i % 4, i < 16.
+//   values   rows = channels, columns = query rows; product step s runs over
+//            tokens 16 s .. 16 s + 15 in the order in which the lane holds their
+//            probabilities, so these never move between lanes.
+// While a page is attended out of one LDS buffer, the next is turned into the
+// other and the one after it is on its way into registers: one barrier a page.
+//
+// What bounds it: a wave's page costs 16 matrix instructions of 32 cycles at
+// head_dim 128, and about as many cycles of vector instructions (16 scores a
+// lane: product with the row's factor, exponential, conversion, maximum, sum;
+// its part of the page's conversion).  Two waves a SIMD run them against each
+// other.  32 rows a wave keep its LDS reads (16 KB a page) under the matrix
+// cores' time.
+#include "kv4_attention.hpp"
+
+namespace sa {
+namespace kv4 {
+namespace {
+
+constexpr int kWaves = 8;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kWaveRows = 32;
+constexpr int kRows = kWaves * kWaveRows;
+constexpr float kShift = 6.0f;  // probabilities are held times 2^6, against a maximum that
+constexpr float kLag = 9.0f;    // may lag by 2^9: below FP16's largest, 2^16
+
+__device__ inline f32x16 mfma32(half8 a, half8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// LDS is handed over; loads from memory stay in flight.
+__device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int D>
+struct Page {
+  using F = Format<D>;
+  half8 k[D / 16][kWave];     // product step, lane of the operand
+  half8 v[D / 32][2][kWave];  // channels' tile, product step, lane
+};
+
+// A thread's part of a page: waves 0..3 keys, 4..7 values.  Wave (tile T of 16
+// tokens = wave % 2, half = wave / 2 % 2), lane (r, j) as in the record:
+//   keys    token 16T + r, the words of half the groups of quarter j
+//   values  tokens 16T + 4j + i, half the channels of row r
+template <int D>
+struct Raw {
+  using F = Format<D>;
+  static constexpr int kKeyWords = F::NG / 2;
+  static constexpr int kValueWords = D == 64 ? 2 : 4;
+  static constexpr int kWords = D == 256 ? 4 : kValueWords;
+  uint32_t codes[kWords];
+  uint32_t s[D == 256 ? 4 : 2];  // keys: a scale a word; values: scales of 4 tokens
+  uint32_t m[2];                 // minima
+};
+
+template <int D>
+__device__ inline void fetch(const uint8_t* rec, int wave, int lane, Raw<D>& x) {
+  using F = Format<D>;
+  const int r = lane % 16, j = lane / 16, T = wave % 2, half = wave / 2 % 2;
+  if (wave < 4) {
+    constexpr int kN = Raw<D>::kKeyWords;
+    const int t = 16 * T + r;
+    const uint8_t* c = rec + t * (D / 2) + (j * F::NG + half * kN) * 4;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      x.codes[i] = reinterpret_cast<const uint32_t*>(c)[i];
+      x.s[i] = *reinterpret_cast<const uint16_t*>(rec + key_scale<D>(t, half * kN + i));
+    }
+    const uint8_t* m = rec + key_min<D>(t, half * kN);
+    if constexpr (kN == 1) {
+      x.m[0] = *reinterpret_cast<const uint16_t*>(m);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kN / 2; ++i) x.m[i] = reinterpret_cast<const uint32_t*>(m)[i];
+    }
+  } else {
+    const uint8_t* c = rec + F::kValueCodes + ((T * 4 + j) * 16 + r) * 2 * F::NC;
+    if constexpr (D == 64) {
+      const uint2 w = *reinterpret_cast<const uint2*>(c);
+      x.codes[0] = w.x, x.codes[1] = w.y;
+    } else if constexpr (D == 128) {
+      const uint4 w = *reinterpret_cast<const uint4*>(c);
+      x.codes[0] = w.x, x.codes[1] = w.y, x.codes[2] = w.z, x.codes[3] = w.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.codes[i] = reinterpret_cast<const uint32_t*>(c)[2 * i + half];
+    }
+    const int meta = (r * F::NC / 32 * 4 + j) * 16 + T * 8;
+    const uint2 s = *reinterpret_cast<const uint2*>(rec + F::kValueScales + meta);
+    const uint2 m = *reinterpret_cast<const uint2*>(rec + F::kValueMins + meta);
+    x.s[0] = s.x, x.s[1] = s.y;
+    x.m[0] = m.x, x.m[1] = m.y;
+  }
+}
+
+__device__ inline uint32_t scaled(half2_t c, half2_t s, half2_t m) { return bits_of(__builtin_elementwise_fma(c, s, m)); }
+
+// Turns the thread's part into operands; returns whether a value's minimum
+// that the sequence holds is NaN.
+template <int D>
+__device__ inline bool convert(const Raw<D>& x, Page<D>& page, int valid, int wave, int lane) {
+  using F = Format<D>;
+  const int r = lane % 16, j = lane / 16, T = wave % 2, half = wave / 2 % 2;
+  if (wave < 4) {
+    constexpr int kN = Raw<D>::kKeyWords;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const uint32_t w = x.codes[i];
+      const half2_t s = as_half2(x.s[i] * 0x10001u);
+      const uint32_t h = i % 2 ? x.m[i / 2] >> 16 : x.m[i / 2] & 0xFFFFu;
+      const half2_t m = as_half2(h * 0x10001u);
+      const int d = j * F::NG + half * kN + i;  // word of the row: channels 32 (d % NG) + 8 (d / NG) ..
+      page.k[d / 2][d % 2 * 32 + 16 * T + r] =
+          as_half8(scaled(low_nibbles(w), s, m), scaled(high_nibbles(w), s, m), scaled(low_nibbles(w >> 8), s, m),
+                   scaled(high_nibbles(w >> 8), s, m));
+    }
+    return false;
+  }
+  uint32_t s[2] = {x.s[0], x.s[1]}, m[2] = {x.m[0], x.m[1]};
+  if (valid < kPageTokens) {  // what lies behind is not the sequence's
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int t = 16 * T + 4 * j + 2 * q;
+      const uint32_t mask = (t < valid ? 0x0000FFFFu : 0u) | (t + 1 < valid ? 0xFFFF0000u : 0u);
+      s[q] &= mask;
+      m[q] &= mask;
+    }
+  }
+  bool nan = false;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) nan |= (m[q] & 0x7fffu) > 0x7c00u || (m[q] >> 16 & 0x7fffu) > 0x7c00u;
+  constexpr int kN = F::NC / 2;  // channels of this half
+#pragma unroll
+  for (int i0 = 0; i0 < kN; i0 += 4) {
+    uint32_t p01, p23;  // 4 nibbles of tokens (0,1) and (2,3)
+    if constexpr (D == 64) {
+      p01 = x.codes[0] >> (half * 8);
+      p23 = x.codes[1] >> (half * 8);
+    } else {
+      const uint32_t sel = (D == 128 ? half == 0 : i0 == 0) ? 0x05040100u : 0x07060302u;
+      p01 = __builtin_amdgcn_perm(x.codes[1], x.codes[0], sel);
+      p23 = __builtin_amdgcn_perm(x.codes[3], x.codes[2], sel);
+    }
+#pragma unroll
+    for (int i = 0; i < (kN < 4 ? kN : 4); ++i) {
+      const uint32_t a = i < 2 ? p01 : p01 >> 8, b = i < 2 ? p23 : p23 >> 8;
+      const half2_t ca = i % 2 ? high_nibbles(a) : low_nibbles(a);
+      const half2_t cb = i % 2 ? high_nibbles(b) : low_nibbles(b);
+      const int n = half * kN + i0 + i;
+      uint2* to = reinterpret_cast<uint2*>(&page.v[n / 2][T][j % 2 * 32 + r + 16 * (n % 2)]) + j / 2;
+      *to = make_uint2(scaled(ca, as_half2(s[0]), as_half2(m[0])), scaled(cb, as_half2(s[1]), as_half2(m[1])));
+    }
+  }
+  return nan;
+}
+
+template <int D>
+struct State {
+  half8 q[D / 16];
+  f32x16 acc[D / 32];
+  float m, l, factor;
+  int limit;        // last position the lane's row sees
+  int first, last;  // of the wave's rows
+  bool huge;
+};
+
+// Adds a page's values token by token, for rows that do not all see every
+// token where some value is NaN: 0 * NaN must not reach a row that does not.
+template <int D>
+__device__ inline void add_each(const Page<D>& page, half8 p0, half8 p1, int valid, int seen, int lane, State<D>& st) {
+#pragma unroll 1
+  for (int t = 0; t < valid; ++t) {
+    const int e = t % 16 / 8 * 4 + t % 4, h = t / 4 % 2;  // slot of the product step t / 16
+    half8 p = t < 16 ? p0 : p1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = i == e && lane / 32 == h ? p[i] : static_cast<_Float16>(0);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      half8 v = page.v[c][t / 16][lane];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i == e && lane / 32 == h ? v[i] : static_cast<_Float16>(0);
+      const f32x16 sum = mfma32(v, p, st.acc[c]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.acc[c][i] = t < seen ? sum[i] : st.acc[c][i];
+    }
+  }
+}
+
+template <int D>
+__device__ inline void attend(const Page<D>& page, const int* nan, int valid, int pos, int lane, State<D>& st) {
+  const int h = lane / 32;
+  f32x16 z{};
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) z = mfma32(page.k[i][lane], st.q[i], z);
+  const bool cut = st.first - pos < kPageTokens - 1;  // some row does not see all of the page
+  int seen = valid;
+  if (cut || valid < kPageTokens) {
+    seen = min(seen, max(st.limit - pos + 1, 0));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 8 * (i / 4) + 4 * h + i % 4 < seen ? z[i] : kLowest;
+  }
+  float top = z[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, z[i]);
+  top *= st.factor;
+  if (__any(top > st.m + kLag)) {
+    top = fmaxf(xor_max<32>(top), st.m);
+    const float f = top > st.m ? __builtin_amdgcn_exp2f(st.m - top) : 1.0f;
+    st.m = top;
+    st.huge |= __any(!(fabsf(top) < 0x1p20f));
+    st.l *= f;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) st.acc[c] *= f;
+  }
+  const float off = kShift - st.m;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float x = __builtin_fmaf(z[i], st.factor, off);
+    if (st.huge) x = z[i] * st.factor + off;
+    z[i] = __builtin_amdgcn_exp2f(x);
+  }
+  if (cut || valid < kPageTokens) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 8 * (i / 4) + 4 * h + i % 4 < seen ? z[i] : 0.0f;
+  }
+  half8 p0, p1;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    p0[i] = static_cast<_Float16>(z[i]);
+    p1[i] = static_cast<_Float16>(z[8 + i]);
+  }
+  // the denominator adds what the numerator multiplies: the rounded ones
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    st.l = __builtin_amdgcn_fdot2(half2_t{p0[i], p0[i + 1]}, half2_t{1, 1}, st.l, false);
+    st.l = __builtin_amdgcn_fdot2(half2_t{p1[i], p1[i + 1]}, half2_t{1, 1}, st.l, false);
+  }
+  if (cut) {
+    int some = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) some |= nan[w];
+    if (__any(some)) {
+      add_each<D>(page, p0, p1, valid, seen, lane, st);
+      return;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    st.acc[c] = mfma32(page.v[c][0][lane], p0, st.acc[c]);
+    st.acc[c] = mfma32(page.v[c][1][lane], p1, st.acc[c]);
+  }
+}
+
+template <int D>
+constexpr int kRecordFloats = kWaves * kWave * (D / 2 + 2);  // a wave's sums, maximum and denominator by lane
+
+template <int D>
+__device__ inline void store_row(const Params& p, int64_t token, int head, const State<D>& st, float l, int h) {
+  constexpr int NC = Format<D>::NC;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {  // row rho = 8 (i / 4) + 4 h + i % 4 of each tile, and rho + 16
+    const int ch = NC * (8 * (i / 4) + 4 * h + i % 4);
+    float x[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) x[n] = l == 0.0f ? 0.0f : st.acc[n / 2][i + 8 * (n % 2)] / l;
+    const int64_t at = (token * p.query_heads + head) * D + ch;
+    if constexpr (NC == 4) {
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+          make_uint2(pack2(x[0], x[1], p.type), pack2(x[2], x[3], p.type));
+    } else {
+#pragma unroll
+      for (int n = 0; n < NC; n += 8)
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at + n) =
+            make_uint4(pack2(x[n], x[n + 1], p.type), pack2(x[n + 2], x[n + 3], p.type),
+                       pack2(x[n + 4], x[n + 5], p.type), pack2(x[n + 6], x[n + 7], p.type));
+    }
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p) {
+  using F = Format<D>;
+  __shared__ Page<D> s_page[2];
+  __shared__ int s_nan[2][4];
+  __shared__ int s_last;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  const int h = lane / 32;
+  const int64_t w = blockIdx.x;
+  const int64_t per_head = p.tile_info[1];
+  const int tiles = static_cast<int>(p.tile_info[0]);
+  Share sh{per_head * p.kv_heads, 0};
+  if (sh.units <= 0) return;
+  sh.groups = min<int64_t>(gridDim.x, max<int64_t>(1, sh.units / kMinUnits));
+  if (w >= sh.groups) return;
+  int64_t u = sh.begin(w);
+  const int64_t end = sh.begin(w + 1);
+  int s = 0;
+  {
+    const int64_t at = u % per_head;
+    int hi = tiles;
+    while (hi - s > 1) {
+      const int mid = (s + hi) / 2;
+      if (p.tile_first[mid] <= at) s = mid;
+      else hi = mid;
+    }
+  }
+
+  while (u < end) {
+    const int head = static_cast<int>(u / per_head);
+    const int4 tile = p.tiles[s];
+    const int b = tile.x, row0 = tile.y, pages = tile.z;
+    const int64_t list_first = head * per_head + p.tile_first[s];
+    const int token0 = p.query_start[b];
+    const int n_tokens = p.query_start[b + 1] - token0;
+    const int len = p.seq_len[b];
+    const List L{nullptr, len, 0, 0, (len + kPageTokens - 1) / kPageTokens};
+    const int p0 = static_cast<int>(u - list_first);
+    const int p1 = static_cast<int>(min<int64_t>(pages, p0 + (end - u)));
+    const int rows = min(kRows, n_tokens * p.group - row0);          // of the tile
+    const int mine = min(kWaveRows, rows - wave * kWaveRows);        // of the wave (may be none)
+    const int row = row0 + wave * kWaveRows + lane % 32;
+    const bool live = lane % 32 < mine;
+    const int token = row / p.group, qh = head * p.group + row % p.group;
+
+    State<D> st;
+    st.m = kNegInf;
+    st.l = 0.0f;
+    st.huge = false;
+    st.limit = len - n_tokens + (live ? token : n_tokens - 1);
+    st.first = __builtin_amdgcn_readfirstlane(st.limit);
+    st.last = mine > 0 ? __builtin_amdgcn_readlane(st.limit, mine - 1) : -1;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) st.acc[c] = f32x16{};
+    {
+      float top = 0.0f, x[D / 16][8];
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const int d = 2 * i + h;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) x[i][n] = 0.0f;
+        if (live)
+          load8(p.query,
+                static_cast<int64_t>(token0 + token) * p.q_stride + static_cast<int64_t>(qh) * D + 32 * (d % F::NG) +
+                    8 * (d / F::NG),
+                p.type == kF16 ? kF16 : kBF16, x[i]);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) top = fmaxf(top, fabsf(x[i][n]));
+      }
+      top = xor_max<32>(top);
+      const int e = top > 0.0f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+      st.factor = ldexp2(fabsf(p.qscale), e);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const float v = x[i][n / 2 + (n % 2) * 4];  // operand order (0,4), (1,5), ...
+          st.q[i][n] = static_cast<_Float16>(ldexp2(p.qscale < 0.0f ? -v : v, -e));
+        }
+    }
+
+    const int64_t page_bytes = static_cast<int64_t>(p.kv_heads) * F::kRecord;
+    const uint8_t* pool = p.pool + static_cast<int64_t>(head) * F::kRecord;
+    PageRef ref{0, 0};
+    int looked = p0 - kWave;  // the lanes hold pages [looked, looked + 64)
+    Raw<D> raw;
+    const auto get = [&](int i) {  // page i into registers; its valid tokens
+      if (i - looked >= kWave) {
+        looked = i;
+        ref = PageRef{0, 0};
+        if (i + lane < p1) ref = resolve(p, b, L, i + lane);
+      }
+      const int64_t page = __builtin_amdgcn_readlane(ref.page, i - looked);
+      fetch<D>(pool + page * page_bytes, wave, lane, raw);
+      return __builtin_amdgcn_readlane(ref.valid, i - looked);
+    };
+    const auto put = [&](int buffer, int valid) {
+      const bool nan = convert<D>(raw, s_page[buffer], valid, wave, lane);
+      if (wave >= 4) {
+        const int any = __any(nan);
+        if (lane == 0) s_nan[buffer][wave - 4] = any;
+      }
+    };
+
+    int valid = get(p0), next = 0;
+    put(0, valid);
+    if (p0 + 1 < p1) next = get(p0 + 1);
+    lds_barrier();
+    for (int i = p0; i < p1; ++i) {
+      const int buffer = (i - p0) % 2;
+      int after = 0;
+      if (i + 1 < p1) {
+        put(buffer ^ 1, next);
+        if (i + 2 < p1) after = get(i + 2);
+      }
+      const int pos = i * kPageTokens;
+      if (valid > 0 && pos <= st.last) attend<D>(s_page[buffer], s_nan[buffer], valid, pos, lane, st);
+      valid = next;
+      next = after;
+      lds_barrier();
+    }
+    st.l = xor_sum<32>(st.l);
+
+    const bool whole = p0 == 0 && p1 == pages;
+    if (whole) {
+      if (live) store_row<D>(p, token0 + token, qh, st, st.l, h);
+    } else {
+      const int64_t w0 = sh.owner(list_first), w1 = sh.owner(list_first + pages - 1);
+      const int shares = static_cast<int>(w1 - w0 + 1);
+      const auto record = [&](int64_t g, bool first) {
+        return p.records + (2 * g + (first ? 1 : 0)) * static_cast<int64_t>(kRecordFloats<D>) +
+               wave * kWave * (D / 2 + 2) + lane;
+      };
+      float* rec = record(w, p0 == 0);
+      store_agent(rec, st.m);
+      store_agent(rec + kWave, st.l);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) store_agent(rec + (2 + c * 16 + i) * kWave, st.acc[c][i]);
+      if (last_arrival(p.arrive + w0, shares, &s_last) && mine > 0) {
+        float top = kNegInf, sum = 0.0f;
+        for (int g = 0; g < shares; ++g) top = fmaxf(top, load_agent(record(w0 + g, g == 0)));
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) st.acc[c] = f32x16{};
+#pragma unroll 1
+        for (int g = 0; g < shares; ++g) {
+          const float* y = record(w0 + g, g == 0);
+          const float m = load_agent(y), l = load_agent(y + kWave);
+          const float f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+          sum = __builtin_fmaf(l, f, sum);
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              st.acc[c][i] = __builtin_fmaf(load_agent(y + (2 + c * 16 + i) * kWave), f, st.acc[c][i]);
+        }
+        if (live) store_row<D>(p, token0 + token, qh, st, sum, h);
+      }
+    }
+    u = list_first + p1;
+    if (p1 == pages && ++s == tiles) s = 0;
+  }
+}
+
+}  // namespace
+
+int prompt_tile_rows(int) { return kRows; }
+int prompt_groups(int) { return compute_units() < kMaxGroups ? compute_units() : kMaxGroups; }
+size_t prompt_record_floats(int head_dim) { return static_cast<size_t>(kWaves) * kWave * (head_dim / 2 + 2); }
+
+hipError_t launch_prompt_tiles(const Params& p, int head_dim, hipStream_t stream) {
+  const dim3 grid(prompt_groups(head_dim));
+  if (head_dim == 64) hipLaunchKernelGGL(kv4_prompt_kernel<64>, grid, dim3(kThreads), 0, stream, p);
+  if (head_dim == 128) hipLaunchKernelGGL(kv4_prompt_kernel<128>, grid, dim3(kThreads), 0, stream, p);
+  if (head_dim == 256) hipLaunchKernelGGL(kv4_prompt_kernel<256>, grid, dim3(kThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace kv4
+}  // namespace sa
