@@ -34,6 +34,8 @@ constexpr int kRows = kWaves * kWaveRows;
 constexpr float kShift = 6.0f;  // probabilities are held times 2^6, against a maximum that
 constexpr float kLag = 9.0f;    // may lag by 2^9: below FP16's largest, 2^16
 
+typedef float float2_t __attribute__((ext_vector_type(2)));
+
 __device__ inline f32x16 mfma32(half8 a, half8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
@@ -46,6 +48,7 @@ struct Page {
   using F = Format<D>;
   half8 k[D / 16][kWave];     // product step, lane of the operand
   half8 v[D / 32][2][kWave];  // channels' tile, product step, lane
+  uint32_t nan[2][F::NG];     // bit t: token 16 T + t of the values' group is NaN
 };
 
 // A thread's part of a page: waves 0..3 keys, 4..7 values.  Wave (tile T of 16
@@ -105,10 +108,11 @@ __device__ inline void fetch(const uint8_t* rec, int wave, int lane, Raw<D>& x) 
 
 __device__ inline uint32_t scaled(half2_t c, half2_t s, half2_t m) { return bits_of(__builtin_elementwise_fma(c, s, m)); }
 
-// Turns the thread's part into operands; returns whether a value's minimum
-// that the sequence holds is NaN.
+// Turns the thread's part into operands.  A NaN minimum of the values goes
+// into page.nan instead (0 * NaN would reach the rows that do not see the
+// token) and its group enters as 0.
 template <int D>
-__device__ inline bool convert(const Raw<D>& x, Page<D>& page, int valid, int wave, int lane) {
+__device__ inline void convert(const Raw<D>& x, Page<D>& page, int valid, int wave, int lane) {
   using F = Format<D>;
   const int r = lane % 16, j = lane / 16, T = wave % 2, half = wave / 2 % 2;
   if (wave < 4) {
@@ -124,7 +128,7 @@ __device__ inline bool convert(const Raw<D>& x, Page<D>& page, int valid, int wa
           as_half8(scaled(low_nibbles(w), s, m), scaled(high_nibbles(w), s, m), scaled(low_nibbles(w >> 8), s, m),
                    scaled(high_nibbles(w >> 8), s, m));
     }
-    return false;
+    return;
   }
   uint32_t s[2] = {x.s[0], x.s[1]}, m[2] = {x.m[0], x.m[1]};
   if (valid < kPageTokens) {  // what lies behind is not the sequence's
@@ -136,9 +140,19 @@ __device__ inline bool convert(const Raw<D>& x, Page<D>& page, int valid, int wa
       m[q] &= mask;
     }
   }
-  bool nan = false;
+  uint32_t nan = 0;  // bit i: token 4j + i of the tile
 #pragma unroll
-  for (int q = 0; q < 2; ++q) nan |= (m[q] & 0x7fffu) > 0x7c00u || (m[q] >> 16 & 0x7fffu) > 0x7c00u;
+  for (int q = 0; q < 2; ++q) {
+    const bool lo = (m[q] & 0x7fffu) > 0x7c00u, hi = (m[q] >> 16 & 0x7fffu) > 0x7c00u;
+    nan |= (lo ? 1u << 2 * q : 0u) | (hi ? 2u << 2 * q : 0u);
+    m[q] &= (lo ? 0xFFFF0000u : ~0u) & (hi ? 0x0000FFFFu : ~0u);
+  }
+  if (__any(nan != 0)) {
+    nan <<= 4 * j;
+    nan |= __shfl_xor(nan, 16);
+    nan |= __shfl_xor(nan, 32);
+  }
+  if (half == 0 && j == 0 && r * F::NC % 32 == 0) page.nan[T][r * F::NC / 32] = nan;
   constexpr int kN = F::NC / 2;  // channels of this half
 #pragma unroll
   for (int i0 = 0; i0 < kN; i0 += 4) {
@@ -161,7 +175,6 @@ __device__ inline bool convert(const Raw<D>& x, Page<D>& page, int valid, int wa
       *to = make_uint2(scaled(ca, as_half2(s[0]), as_half2(m[0])), scaled(cb, as_half2(s[1]), as_half2(m[1])));
     }
   }
-  return nan;
 }
 
 template <int D>
@@ -174,30 +187,8 @@ struct State {
   bool huge;
 };
 
-// Adds a page's values token by token, for rows that do not all see every
-// token where some value is NaN: 0 * NaN must not reach a row that does not.
 template <int D>
-__device__ inline void add_each(const Page<D>& page, half8 p0, half8 p1, int valid, int seen, int lane, State<D>& st) {
-#pragma unroll 1
-  for (int t = 0; t < valid; ++t) {
-    const int e = t % 16 / 8 * 4 + t % 4, h = t / 4 % 2;  // slot of the product step t / 16
-    half8 p = t < 16 ? p0 : p1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = i == e && lane / 32 == h ? p[i] : static_cast<_Float16>(0);
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      half8 v = page.v[c][t / 16][lane];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i == e && lane / 32 == h ? v[i] : static_cast<_Float16>(0);
-      const f32x16 sum = mfma32(v, p, st.acc[c]);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) st.acc[c][i] = t < seen ? sum[i] : st.acc[c][i];
-    }
-  }
-}
-
-template <int D>
-__device__ inline void attend(const Page<D>& page, const int* nan, int valid, int pos, int lane, State<D>& st) {
+__device__ inline void attend(const Page<D>& page, int valid, int pos, int lane, State<D>& st) {
   const int h = lane / 32;
   f32x16 z{};
 #pragma unroll
@@ -233,31 +224,32 @@ __device__ inline void attend(const Page<D>& page, const int* nan, int valid, in
 #pragma unroll
     for (int i = 0; i < 16; ++i) z[i] = 8 * (i / 4) + 4 * h + i % 4 < seen ? z[i] : 0.0f;
   }
-  half8 p0, p1;
+  // the denominator adds what the numerator multiplies: the rounded ones
+  uint32_t pairs[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    p0[i] = static_cast<_Float16>(z[i]);
-    p1[i] = static_cast<_Float16>(z[8 + i]);
+    const half2_t pair = __builtin_convertvector(float2_t{z[2 * i], z[2 * i + 1]}, half2_t);
+    st.l = __builtin_amdgcn_fdot2(pair, half2_t{1, 1}, st.l, false);
+    pairs[i] = bits_of(pair);
   }
-  // the denominator adds what the numerator multiplies: the rounded ones
-#pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    st.l = __builtin_amdgcn_fdot2(half2_t{p0[i], p0[i + 1]}, half2_t{1, 1}, st.l, false);
-    st.l = __builtin_amdgcn_fdot2(half2_t{p1[i], p1[i + 1]}, half2_t{1, 1}, st.l, false);
-  }
-  if (cut) {
-    int some = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) some |= nan[w];
-    if (__any(some)) {
-      add_each<D>(page, p0, p1, valid, seen, lane, st);
-      return;
-    }
-  }
+  const half8 p0 = as_half8(pairs[0], pairs[1], pairs[2], pairs[3]);
+  const half8 p1 = as_half8(pairs[4], pairs[5], pairs[6], pairs[7]);
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
     st.acc[c] = mfma32(page.v[c][0][lane], p0, st.acc[c]);
     st.acc[c] = mfma32(page.v[c][1][lane], p1, st.acc[c]);
+  }
+  constexpr int kNG = Format<D>::NG, kNC = Format<D>::NC;
+  if (__any(lane < 2 * kNG && page.nan[lane / kNG % 2][lane % kNG] != 0)) {
+    const uint32_t sees = seen >= 32 ? ~0u : (1u << seen) - 1u;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {  // channel NC (8 (i / 4) + 4 h + i % 4) + .. of rows 0..15, and again 16..31
+      const int g = (8 * (i / 4 % 2) + 4 * h + i % 4) * kNC / 32;
+      if ((page.nan[0][g] | page.nan[1][g] << 16) & sees) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) st.acc[c][i] = __builtin_nanf("");
+      }
+    }
   }
 }
 
@@ -291,7 +283,6 @@ template <int D>
 __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p) {
   using F = Format<D>;
   __shared__ Page<D> s_page[2];
-  __shared__ int s_nan[2][4];
   __shared__ int s_last;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
@@ -367,6 +358,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
           const float v = x[i][n / 2 + (n % 2) * 4];  // operand order (0,4), (1,5), ...
           st.q[i][n] = static_cast<_Float16>(ldexp2(p.qscale < 0.0f ? -v : v, -e));
         }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(st.q[i]));  // made once, not anew for every page
     }
 
     const int64_t page_bytes = static_cast<int64_t>(p.kv_heads) * F::kRecord;
@@ -384,13 +377,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
       fetch<D>(pool + page * page_bytes, wave, lane, raw);
       return __builtin_amdgcn_readlane(ref.valid, i - looked);
     };
-    const auto put = [&](int buffer, int valid) {
-      const bool nan = convert<D>(raw, s_page[buffer], valid, wave, lane);
-      if (wave >= 4) {
-        const int any = __any(nan);
-        if (lane == 0) s_nan[buffer][wave - 4] = any;
-      }
-    };
+    const auto put = [&](int buffer, int valid) { convert<D>(raw, s_page[buffer], valid, wave, lane); };
 
     int valid = get(p0), next = 0;
     put(0, valid);
@@ -404,7 +391,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
         if (i + 2 < p1) after = get(i + 2);
       }
       const int pos = i * kPageTokens;
-      if (valid > 0 && pos <= st.last) attend<D>(s_page[buffer], s_nan[buffer], valid, pos, lane, st);
+      if (valid > 0 && pos <= st.last) attend<D>(s_page[buffer], valid, pos, lane, st);
       valid = next;
       next = after;
       lds_barrier();
