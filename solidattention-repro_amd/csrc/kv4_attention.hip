@@ -791,14 +791,14 @@ struct Plan {
 
 Plan plan(Form form, int head_dim) {
   if (form == Form::kMany)
-    return {prompt_tile_rows(head_dim), 2 * prompt_groups(head_dim) * prompt_record_floats(head_dim) * sizeof(float)};
+    return {prompt_tile_rows(), 2 * prompt_groups() * prompt_record_floats(head_dim) * sizeof(float)};
   const int RT = form == Form::kFew && head_dim <= 128 ? 2 : 1;
   return {rows_of(RT), 2 * grid_groups(head_dim, RT) * record_floats(head_dim, rows_of(RT)) * sizeof(float)};
 }
 
-Form form_of(bool prompt, int64_t tokens, int64_t batch, int group, int type) {
+Form form_of(bool prompt, int64_t tokens, int64_t batch, int group, int head_dim, int type) {
   if (!prompt) return Form::kDecode;
-  return type != kF32 && tokens * group >= 64 * batch ? Form::kMany : Form::kFew;
+  return type != kF32 && head_dim <= 128 && tokens * group >= 64 * batch ? Form::kMany : Form::kFew;
 }
 
 struct Layout {
@@ -881,7 +881,7 @@ hipError_t launch_kv4_attention(const Kv4AttnLaunch& a, hipStream_t stream) {
   p.group = a.query_heads / a.kv_heads;
   p.type = a.type;
   p.qscale = a.scale * kLog2e;
-  const Form form = form_of(a.query_start != nullptr, a.tokens, a.batch, p.group, a.type);
+  const Form form = form_of(a.query_start != nullptr, a.tokens, a.batch, p.group, a.head_dim, a.type);
   const Plan pl = plan(form, a.head_dim);
   const Layout l = layout(pl, a.batch, a.tokens, p.group);
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);

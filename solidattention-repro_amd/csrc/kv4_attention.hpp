@@ -186,10 +186,10 @@ struct Target {
 hipError_t launch_tiles(const Params& p, int rows, hipStream_t stream);
 int64_t max_tiles(int64_t batch, int64_t tokens, int group, int rows);
 
-// Tiles of many rows (kv4_prompt.hip): rows of a tile, workgroups of a launch,
-// floats of one of its two records a workgroup.
-int prompt_tile_rows(int head_dim);
-int prompt_groups(int head_dim);
+// Tiles of many rows (kv4_prompt.hip; head_dim 64 and 128): rows of a tile,
+// workgroups of a launch, floats of one of its two records a workgroup.
+int prompt_tile_rows();
+int prompt_groups();
 size_t prompt_record_floats(int head_dim);
 hipError_t launch_prompt_tiles(const Params& p, int head_dim, hipStream_t stream);
 

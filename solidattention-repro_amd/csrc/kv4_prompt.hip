@@ -12,8 +12,11 @@
 //   values   rows = channels, columns = query rows; product step s runs over
 //            tokens 16 s .. 16 s + 15 in the order in which the lane holds their
 //            probabilities, so these never move between lanes.
-// While a page is attended out of one LDS buffer, the next is turned into the
-// other and the one after it is on its way into registers: one barrier a page.
+// While up to four pages are attended out of one set of LDS buffers, the next
+// four are turned into the other, each on its way into registers before: one
+// barrier every four pages.  Of the two waves of a SIMD one converts a page and
+// then attends one, the other attends first, so that one's matrix instructions
+// meet the other's vector instructions.
 //
 // What bounds it: a wave's page costs 16 matrix instructions of 32 cycles at
 // head_dim 128, and about as many cycles of vector instructions (16 scores a
@@ -49,7 +52,10 @@ struct Page {
   half8 k[D / 16][kWave];     // product step, lane of the operand
   half8 v[D / 32][2][kWave];  // channels' tile, product step, lane
   uint32_t nan[2][F::NG];     // bit t: token 16 T + t of the values' group is NaN
+  int valid;                  // tokens (0: no page)
 };
+
+constexpr int kBatch = 4;  // pages of a set: two sets fit the LDS of a compute unit
 
 // A thread's part of a page: waves 0..3 keys, 4..7 values.  Wave (tile T of 16
 // tokens = wave % 2, half = wave / 2 % 2), lane (r, j) as in the record:
@@ -59,11 +65,9 @@ template <int D>
 struct Raw {
   using F = Format<D>;
   static constexpr int kKeyWords = F::NG / 2;
-  static constexpr int kValueWords = D == 64 ? 2 : 4;
-  static constexpr int kWords = D == 256 ? 4 : kValueWords;
-  uint32_t codes[kWords];
-  uint32_t s[D == 256 ? 4 : 2];  // keys: a scale a word; values: scales of 4 tokens
-  uint32_t m[2];                 // minima
+  uint32_t codes[D == 64 ? 2 : 4];
+  uint32_t s[2];  // keys: a scale a word; values: scales of 4 tokens
+  uint32_t m[2];  // minima
 };
 
 template <int D>
@@ -80,23 +84,18 @@ __device__ inline void fetch(const uint8_t* rec, int wave, int lane, Raw<D>& x) 
       x.s[i] = *reinterpret_cast<const uint16_t*>(rec + key_scale<D>(t, half * kN + i));
     }
     const uint8_t* m = rec + key_min<D>(t, half * kN);
-    if constexpr (kN == 1) {
+    if constexpr (kN == 1)
       x.m[0] = *reinterpret_cast<const uint16_t*>(m);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kN / 2; ++i) x.m[i] = reinterpret_cast<const uint32_t*>(m)[i];
-    }
+    else
+      x.m[0] = *reinterpret_cast<const uint32_t*>(m);
   } else {
     const uint8_t* c = rec + F::kValueCodes + ((T * 4 + j) * 16 + r) * 2 * F::NC;
     if constexpr (D == 64) {
       const uint2 w = *reinterpret_cast<const uint2*>(c);
       x.codes[0] = w.x, x.codes[1] = w.y;
-    } else if constexpr (D == 128) {
+    } else {
       const uint4 w = *reinterpret_cast<const uint4*>(c);
       x.codes[0] = w.x, x.codes[1] = w.y, x.codes[2] = w.z, x.codes[3] = w.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x.codes[i] = reinterpret_cast<const uint32_t*>(c)[2 * i + half];
     }
     const int meta = (r * F::NC / 32 * 4 + j) * 16 + T * 8;
     const uint2 s = *reinterpret_cast<const uint2*>(rec + F::kValueScales + meta);
@@ -116,12 +115,13 @@ __device__ inline void convert(const Raw<D>& x, Page<D>& page, int valid, int wa
   using F = Format<D>;
   const int r = lane % 16, j = lane / 16, T = wave % 2, half = wave / 2 % 2;
   if (wave < 4) {
+    if (wave == 0 && lane == 0) page.valid = valid;
     constexpr int kN = Raw<D>::kKeyWords;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const uint32_t w = x.codes[i];
       const half2_t s = as_half2(x.s[i] * 0x10001u);
-      const uint32_t h = i % 2 ? x.m[i / 2] >> 16 : x.m[i / 2] & 0xFFFFu;
+      const uint32_t h = i % 2 ? x.m[0] >> 16 : x.m[0] & 0xFFFFu;
       const half2_t m = as_half2(h * 0x10001u);
       const int d = j * F::NG + half * kN + i;  // word of the row: channels 32 (d % NG) + 8 (d / NG) ..
       page.k[d / 2][d % 2 * 32 + 16 * T + r] =
@@ -141,13 +141,14 @@ __device__ inline void convert(const Raw<D>& x, Page<D>& page, int valid, int wa
     }
   }
   uint32_t nan = 0;  // bit i: token 4j + i of the tile
+  const half2_t zero{0, 0};  // a minimum is finite or NaN: its product with 0 is 0 or NaN
+  if (__any(((bits_of(as_half2(m[0]) * zero) | bits_of(as_half2(m[1]) * zero)) & 0x7FFF7FFFu) != 0)) {
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const bool lo = (m[q] & 0x7fffu) > 0x7c00u, hi = (m[q] >> 16 & 0x7fffu) > 0x7c00u;
-    nan |= (lo ? 1u << 2 * q : 0u) | (hi ? 2u << 2 * q : 0u);
-    m[q] &= (lo ? 0xFFFF0000u : ~0u) & (hi ? 0x0000FFFFu : ~0u);
-  }
-  if (__any(nan != 0)) {
+    for (int q = 0; q < 2; ++q) {
+      const bool lo = (m[q] & 0x7fffu) > 0x7c00u, hi = (m[q] >> 16 & 0x7fffu) > 0x7c00u;
+      nan |= (lo ? 1u << 2 * q : 0u) | (hi ? 2u << 2 * q : 0u);
+      m[q] &= (lo ? 0xFFFF0000u : ~0u) & (hi ? 0x0000FFFFu : ~0u);
+    }
     nan <<= 4 * j;
     nan |= __shfl_xor(nan, 16);
     nan |= __shfl_xor(nan, 32);
@@ -161,7 +162,7 @@ __device__ inline void convert(const Raw<D>& x, Page<D>& page, int valid, int wa
       p01 = x.codes[0] >> (half * 8);
       p23 = x.codes[1] >> (half * 8);
     } else {
-      const uint32_t sel = (D == 128 ? half == 0 : i0 == 0) ? 0x05040100u : 0x07060302u;
+      const uint32_t sel = half == 0 ? 0x05040100u : 0x07060302u;
       p01 = __builtin_amdgcn_perm(x.codes[1], x.codes[0], sel);
       p23 = __builtin_amdgcn_perm(x.codes[3], x.codes[2], sel);
     }
@@ -190,9 +191,20 @@ struct State {
 template <int D>
 __device__ inline void attend(const Page<D>& page, int valid, int pos, int lane, State<D>& st) {
   const int h = lane / 32;
+  // The operands are read ahead of the products that take them, the values'
+  // before the exponentials: read one by one, the LDS's latency took more
+  // than half of the time.
+  half8 op[D / 16];
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) op[i] = page.k[i][lane];
+  __builtin_amdgcn_sched_barrier(0);
   f32x16 z{};
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) z = mfma32(page.k[i][lane], st.q[i], z);
+  for (int i = 0; i < D / 16; ++i) z = mfma32(op[i], st.q[i], z);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) op[i] = page.v[i / 2][i % 2][lane];
+  __builtin_amdgcn_sched_barrier(0);
   const bool cut = st.first - pos < kPageTokens - 1;  // some row does not see all of the page
   int seen = valid;
   if (cut || valid < kPageTokens) {
@@ -236,8 +248,8 @@ __device__ inline void attend(const Page<D>& page, int valid, int pos, int lane,
   const half8 p1 = as_half8(pairs[4], pairs[5], pairs[6], pairs[7]);
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
-    st.acc[c] = mfma32(page.v[c][0][lane], p0, st.acc[c]);
-    st.acc[c] = mfma32(page.v[c][1][lane], p1, st.acc[c]);
+    st.acc[c] = mfma32(op[2 * c], p0, st.acc[c]);
+    st.acc[c] = mfma32(op[2 * c + 1], p1, st.acc[c]);
   }
   constexpr int kNG = Format<D>::NG, kNC = Format<D>::NC;
   if (__any(lane < 2 * kNG && page.nan[lane / kNG % 2][lane % kNG] != 0)) {
@@ -282,7 +294,7 @@ __device__ inline void store_row(const Params& p, int64_t token, int head, const
 template <int D>
 __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p) {
   using F = Format<D>;
-  __shared__ Page<D> s_page[2];
+  __shared__ Page<D> s_page[2][kBatch];
   __shared__ int s_last;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
@@ -377,24 +389,32 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
       fetch<D>(pool + page * page_bytes, wave, lane, raw);
       return __builtin_amdgcn_readlane(ref.valid, i - looked);
     };
-    const auto put = [&](int buffer, int valid) { convert<D>(raw, s_page[buffer], valid, wave, lane); };
-
-    int valid = get(p0), next = 0;
-    put(0, valid);
-    if (p0 + 1 < p1) next = get(p0 + 1);
-    lds_barrier();
-    for (int i = p0; i < p1; ++i) {
-      const int buffer = (i - p0) % 2;
-      int after = 0;
-      if (i + 1 < p1) {
-        put(buffer ^ 1, next);
-        if (i + 2 < p1) after = get(i + 2);
-      }
+    int raw_valid = get(p0);
+    const auto put = [&](int i, Page<D>& page) {  // page i, which is in registers; then the next one into them
+      convert<D>(raw, page, raw_valid, wave, lane);
+      if (i + 1 < p1) raw_valid = get(i + 1);
+    };
+    const auto use = [&](int i, const Page<D>& page) {
       const int pos = i * kPageTokens;
-      if (valid > 0 && pos <= st.last) attend<D>(s_page[buffer], valid, pos, lane, st);
-      valid = next;
-      next = after;
+      if (pos > st.last) return;
+      const int valid = __builtin_amdgcn_readfirstlane(page.valid);
+      if (valid > 0) attend<D>(page, valid, pos, lane, st);
+    };
+    // [a, z) are attended out of one set while [z, y) go into the other; sets
+    // grow from one page, so that the first is not waited for longer.  (One
+    // place in the code for each: two would copy the sums between them.)
+    put(p0, s_page[0][0]);
+    lds_barrier();
+    const int late = wave / (kWaves / 2);
+    for (int a = p0, z = p0 + 1, set = 0; a < p1; set ^= 1) {
+      const int y = min(p1, z + min(kBatch, 2 * (z - a)));
+      for (int i = 0; i < max(z - a, y - z) + late; ++i) {
+        if (i >= late && z + i - late < y) put(z + i - late, s_page[set ^ 1][i - late]);
+        if (a + i < z) use(a + i, s_page[set][i]);
+      }
       lds_barrier();
+      a = z;
+      z = y;
     }
     st.l = xor_sum<32>(st.l);
 
@@ -442,15 +462,14 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
 
 }  // namespace
 
-int prompt_tile_rows(int) { return kRows; }
-int prompt_groups(int) { return compute_units() < kMaxGroups ? compute_units() : kMaxGroups; }
+int prompt_tile_rows() { return kRows; }
+int prompt_groups() { return compute_units() < kMaxGroups ? compute_units() : kMaxGroups; }
 size_t prompt_record_floats(int head_dim) { return static_cast<size_t>(kWaves) * kWave * (head_dim / 2 + 2); }
 
 hipError_t launch_prompt_tiles(const Params& p, int head_dim, hipStream_t stream) {
-  const dim3 grid(prompt_groups(head_dim));
+  const dim3 grid(prompt_groups());
   if (head_dim == 64) hipLaunchKernelGGL(kv4_prompt_kernel<64>, grid, dim3(kThreads), 0, stream, p);
   if (head_dim == 128) hipLaunchKernelGGL(kv4_prompt_kernel<128>, grid, dim3(kThreads), 0, stream, p);
-  if (head_dim == 256) hipLaunchKernelGGL(kv4_prompt_kernel<256>, grid, dim3(kThreads), 0, stream, p);
   return hipGetLastError();
 }
 

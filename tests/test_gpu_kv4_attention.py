@@ -322,6 +322,41 @@ def test_same_bits_every_time(hip):
         assert torch.equal(hip.kv4_prompt_attention(c.kv, q, start, 0.1), p)
 
 
+@pytest.mark.parametrize("d,heads,group", [(64, 2, 4), (128, 2, 4), (128, 1, 16)])
+def test_long_chunks(hip, d, heads, group):
+    """Chunks of hundreds of rows at contexts of several thousand: tiles over many pages, cut by shares, and the same
+    bits every time; a page that is not there among them."""
+    c = Cache(hip, [3000, 700, 2100], heads, d, group, seed=5)
+    new = [300, 700, 65]
+    start = np.concatenate([[0], np.cumsum(new)])
+    q = query(9, int(start[-1]), heads * group, d, "bf16")
+    ws = hip.kv4_attention_workspace(c.kv, q.shape[0])
+    out = hip.kv4_prompt_attention(c.kv, q.cuda(), ints(start), d ** -0.5, workspace=ws)
+    qn, on = q.double().numpy(), out.double().cpu().numpy()
+    for b, n in enumerate(c.lengths):
+        blocks = np.arange((n + 31) // 32)
+        for h in range(heads):
+            k, v = c.rows(b, h, blocks, n)
+            rows = slice(h * group, (h + 1) * group)
+            for i in list(range(0, new[b], 37)) + [new[b] - 1]:
+                seen = n - new[b] + i + 1
+                qq = qn[start[b] + i, rows]
+                want, _ = K.attend(qq, k[:seen], v[:seen], d ** -0.5)
+                check(on[start[b] + i, rows], want, K.error_bound(qq, k[:seen], v[:seen], d ** -0.5, "bf16",
+                                                                  EPS["bf16"]), (b, h, i))
+    for _ in range(4):
+        assert torch.equal(hip.kv4_prompt_attention(c.kv, q.cuda(), ints(start), d ** -0.5, workspace=ws), out)
+    c.kv.block_table[0, 50] = c.kv.num_pages + 7
+    status = ints([0])
+    on = hip.kv4_prompt_attention(c.kv, q.cuda(), ints(start), d ** -0.5, workspace=ws, status=status).double().cpu().numpy()
+    assert int(status) == 1
+    k, v = c.rows(0, 0, np.array([i for i in range(94) if i != 50]), 3000)
+    for i in (0, 123, 299):
+        seen = 3000 - 300 + i + 1 - 32
+        want, _ = K.attend(qn[i, :group], k[:seen], v[:seen], d ** -0.5)
+        check(on[i, :group], want, K.error_bound(qn[i, :group], k[:seen], v[:seen], d ** -0.5, "bf16", EPS["bf16"]))
+
+
 def test_captured(hip):
     """Both calls in one graph, replayed on new queries and lengths."""
     c = Cache(hip, [600, 90, 333], 2, 128, 2)
