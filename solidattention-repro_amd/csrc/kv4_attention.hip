@@ -323,16 +323,27 @@ __device__ inline void attend(Record<D>& x, int valid, int64_t pos, int64_t firs
       for (int n = 0; n < F::NC; ++n) st.acc[rt][n] *= f;
     }
     const float off = kShift<kFine> - st.m[rt];
+    // one rounding for product and difference: the maximum's own rounding is
+    // the row's common factor, unless it passes the whole range of FP16
+    float e[8];
+    if (__builtin_expect(st.huge, false)) {
+      asm volatile("");  // a branch: as a select it would cost three instructions a score
+#pragma unroll
+      for (int n = 0; n < 8; ++n) e[n] = z[rt][n / 4][n % 4] * q.factor[rt] + off;
+    } else {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) e[n] = __builtin_fmaf(z[rt][n / 4][n % 4], q.factor[rt], off);
+    }
+#pragma unroll
+    for (int n = 0; n < 8; ++n) e[n] = __builtin_amdgcn_exp2f(e[n]);
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) e[n] = 16 * (n / 4) + 4 * j + n % 4 < seen ? e[n] : 0.0f;
+    }
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      // one rounding for product and difference: the maximum's own rounding is
-      // the row's common factor, unless it passes the whole range of FP16
-      float x = __builtin_fmaf(z[rt][n / 4][n % 4], q.factor[rt], off);
-      if (st.huge) x = z[rt][n / 4][n % 4] * q.factor[rt] + off;
-      float v = __builtin_amdgcn_exp2f(x);
-      if (masked) v = 16 * (n / 4) + 4 * j + n % 4 < seen ? v : 0.0f;
-      ph[rt][n] = static_cast<_Float16>(v);
-      if constexpr (kFine) pl[rt][n] = static_cast<_Float16>(v - static_cast<float>(ph[rt][n]));
+      ph[rt][n] = static_cast<_Float16>(e[n]);
+      if constexpr (kFine) pl[rt][n] = static_cast<_Float16>(e[n] - static_cast<float>(ph[rt][n]));
     }
   }
 

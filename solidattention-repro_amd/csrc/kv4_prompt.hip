@@ -52,7 +52,7 @@ struct Page {
   half8 k[D / 16][kWave];     // product step, lane of the operand
   half8 v[D / 32][2][kWave];  // channels' tile, product step, lane
   uint32_t nan[2][F::NG];     // bit t: token 16 T + t of the values' group is NaN
-  int valid;                  // tokens (0: no page)
+  uint32_t valid;             // tokens (0: no page); right behind the words of `nan`
 };
 
 constexpr int kBatch = 4;  // pages of a set: two sets fit the LDS of a compute unit
@@ -70,38 +70,58 @@ struct Raw {
   uint32_t m[2];  // minima
 };
 
+// Where a thread's part lies in a record, whichever it is, and its first place
+// in a Page: 32-bit offsets, so that the records' addresses stay scalar.
 template <int D>
-__device__ inline void fetch(const uint8_t* rec, int wave, int lane, Raw<D>& x) {
-  using F = Format<D>;
-  const int r = lane % 16, j = lane / 16, T = wave % 2, half = wave / 2 % 2;
-  if (wave < 4) {
-    constexpr int kN = Raw<D>::kKeyWords;
-    const int t = 16 * T + r;
-    const uint8_t* c = rec + t * (D / 2) + (j * F::NG + half * kN) * 4;
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      x.codes[i] = reinterpret_cast<const uint32_t*>(c)[i];
-      x.s[i] = *reinterpret_cast<const uint16_t*>(rec + key_scale<D>(t, half * kN + i));
+struct Place {
+  uint32_t codes, s, m, to;
+  __device__ inline Place(int wave, int lane) {
+    using F = Format<D>;
+    const int r = lane % 16, j = lane / 16, T = wave % 2, half = wave / 2 % 2;
+    if (wave < 4) {
+      const int t = 16 * T + r, d = j * F::NG + half * (F::NG / 2);  // first word of the row
+      codes = t * (D / 2) + d * 4;
+      s = key_scale<D>(t, half * (F::NG / 2));
+      m = key_min<D>(t, half * (F::NG / 2));
+      to = (d / 2 * kWave + d % 2 * 32 + t) * 16;
+    } else {
+      codes = F::kValueCodes + ((T * 4 + j) * 16 + r) * 2 * F::NC;
+      s = F::kValueScales + (r * F::NC / 32 * 4 + j) * 16 + T * 8;
+      m = s + (F::kValueMins - F::kValueScales);
+      const int n = half * (F::NC / 2);
+      to = D / 16 * kWave * 16 + ((n / 2 * 2 + T) * kWave + j % 2 * 32 + r) * 16 + j / 2 * 8;
     }
-    const uint8_t* m = rec + key_min<D>(t, half * kN);
-    if constexpr (kN == 1)
-      x.m[0] = *reinterpret_cast<const uint16_t*>(m);
-    else
-      x.m[0] = *reinterpret_cast<const uint32_t*>(m);
-  } else {
-    const uint8_t* c = rec + F::kValueCodes + ((T * 4 + j) * 16 + r) * 2 * F::NC;
+  }
+};
+
+template <int D>
+__device__ inline void fetch(const uint8_t* rec, const Place<D>& at, int wave, Raw<D>& x) {
+  const uint8_t* codes = rec + at.codes;
+  const uint8_t* s = rec + at.s;
+  const uint8_t* m = rec + at.m;
+  if (wave < 4) {
     if constexpr (D == 64) {
-      const uint2 w = *reinterpret_cast<const uint2*>(c);
+      x.codes[0] = *reinterpret_cast<const uint32_t*>(codes);
+      x.s[0] = *reinterpret_cast<const uint16_t*>(s);
+      x.m[0] = *reinterpret_cast<const uint16_t*>(m);
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2*>(codes);
+      x.codes[0] = w.x, x.codes[1] = w.y;
+      x.s[0] = *reinterpret_cast<const uint16_t*>(s);
+      x.s[1] = *reinterpret_cast<const uint16_t*>(s + 8);  // the next group's
+      x.m[0] = *reinterpret_cast<const uint32_t*>(m);
+    }
+  } else {
+    if constexpr (D == 64) {
+      const uint2 w = *reinterpret_cast<const uint2*>(codes);
       x.codes[0] = w.x, x.codes[1] = w.y;
     } else {
-      const uint4 w = *reinterpret_cast<const uint4*>(c);
+      const uint4 w = *reinterpret_cast<const uint4*>(codes);
       x.codes[0] = w.x, x.codes[1] = w.y, x.codes[2] = w.z, x.codes[3] = w.w;
     }
-    const int meta = (r * F::NC / 32 * 4 + j) * 16 + T * 8;
-    const uint2 s = *reinterpret_cast<const uint2*>(rec + F::kValueScales + meta);
-    const uint2 m = *reinterpret_cast<const uint2*>(rec + F::kValueMins + meta);
-    x.s[0] = s.x, x.s[1] = s.y;
-    x.m[0] = m.x, x.m[1] = m.y;
+    const uint2 a = *reinterpret_cast<const uint2*>(s), b = *reinterpret_cast<const uint2*>(m);
+    x.s[0] = a.x, x.s[1] = a.y;
+    x.m[0] = b.x, x.m[1] = b.y;
   }
 }
 
@@ -111,20 +131,18 @@ __device__ inline uint32_t scaled(half2_t c, half2_t s, half2_t m) { return bits
 // into page.nan instead (0 * NaN would reach the rows that do not see the
 // token) and its group enters as 0.
 template <int D>
-__device__ inline void convert(const Raw<D>& x, Page<D>& page, int valid, int wave, int lane) {
+__device__ inline void convert(const Raw<D>& x, Page<D>& page, int valid, const Place<D>& at, int wave, int lane) {
   using F = Format<D>;
   const int r = lane % 16, j = lane / 16, T = wave % 2, half = wave / 2 % 2;
+  uint8_t* to = reinterpret_cast<uint8_t*>(&page) + at.to;
   if (wave < 4) {
     if (wave == 0 && lane == 0) page.valid = valid;
-    constexpr int kN = Raw<D>::kKeyWords;
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
+    for (int i = 0; i < F::NG / 2; ++i) {  // the row's next word is the other half of a product step
       const uint32_t w = x.codes[i];
       const half2_t s = as_half2(x.s[i] * 0x10001u);
-      const uint32_t h = i % 2 ? x.m[0] >> 16 : x.m[0] & 0xFFFFu;
-      const half2_t m = as_half2(h * 0x10001u);
-      const int d = j * F::NG + half * kN + i;  // word of the row: channels 32 (d % NG) + 8 (d / NG) ..
-      page.k[d / 2][d % 2 * 32 + 16 * T + r] =
+      const half2_t m = as_half2((i % 2 ? x.m[0] >> 16 : x.m[0] & 0xFFFFu) * 0x10001u);
+      *reinterpret_cast<half8*>(to + i * 32 * 16) =
           as_half8(scaled(low_nibbles(w), s, m), scaled(high_nibbles(w), s, m), scaled(low_nibbles(w >> 8), s, m),
                    scaled(high_nibbles(w >> 8), s, m));
     }
@@ -143,6 +161,7 @@ __device__ inline void convert(const Raw<D>& x, Page<D>& page, int valid, int wa
   uint32_t nan = 0;  // bit i: token 4j + i of the tile
   const half2_t zero{0, 0};  // a minimum is finite or NaN: its product with 0 is 0 or NaN
   if (__any(((bits_of(as_half2(m[0]) * zero) | bits_of(as_half2(m[1]) * zero)) & 0x7FFF7FFFu) != 0)) {
+    asm volatile("");
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const bool lo = (m[q] & 0x7fffu) > 0x7c00u, hi = (m[q] >> 16 & 0x7fffu) > 0x7c00u;
@@ -154,27 +173,22 @@ __device__ inline void convert(const Raw<D>& x, Page<D>& page, int valid, int wa
     nan |= __shfl_xor(nan, 32);
   }
   if (half == 0 && j == 0 && r * F::NC % 32 == 0) page.nan[T][r * F::NC / 32] = nan;
-  constexpr int kN = F::NC / 2;  // channels of this half
+  uint32_t p01, p23;  // 4 nibbles of tokens (0,1) and (2,3)
+  if constexpr (D == 64) {
+    p01 = x.codes[0] >> (half * 8);
+    p23 = x.codes[1] >> (half * 8);
+  } else {
+    const uint32_t sel = half == 0 ? 0x05040100u : 0x07060302u;
+    p01 = __builtin_amdgcn_perm(x.codes[1], x.codes[0], sel);
+    p23 = __builtin_amdgcn_perm(x.codes[3], x.codes[2], sel);
+  }
 #pragma unroll
-  for (int i0 = 0; i0 < kN; i0 += 4) {
-    uint32_t p01, p23;  // 4 nibbles of tokens (0,1) and (2,3)
-    if constexpr (D == 64) {
-      p01 = x.codes[0] >> (half * 8);
-      p23 = x.codes[1] >> (half * 8);
-    } else {
-      const uint32_t sel = half == 0 ? 0x05040100u : 0x07060302u;
-      p01 = __builtin_amdgcn_perm(x.codes[1], x.codes[0], sel);
-      p23 = __builtin_amdgcn_perm(x.codes[3], x.codes[2], sel);
-    }
-#pragma unroll
-    for (int i = 0; i < (kN < 4 ? kN : 4); ++i) {
-      const uint32_t a = i < 2 ? p01 : p01 >> 8, b = i < 2 ? p23 : p23 >> 8;
-      const half2_t ca = i % 2 ? high_nibbles(a) : low_nibbles(a);
-      const half2_t cb = i % 2 ? high_nibbles(b) : low_nibbles(b);
-      const int n = half * kN + i0 + i;
-      uint2* to = reinterpret_cast<uint2*>(&page.v[n / 2][T][j % 2 * 32 + r + 16 * (n % 2)]) + j / 2;
-      *to = make_uint2(scaled(ca, as_half2(s[0]), as_half2(m[0])), scaled(cb, as_half2(s[1]), as_half2(m[1])));
-    }
+  for (int i = 0; i < F::NC / 2; ++i) {
+    const uint32_t a = i < 2 ? p01 : p01 >> 8, b = i < 2 ? p23 : p23 >> 8;
+    const half2_t ca = i % 2 ? high_nibbles(a) : low_nibbles(a);
+    const half2_t cb = i % 2 ? high_nibbles(b) : low_nibbles(b);
+    *reinterpret_cast<uint2*>(to + (i / 2 * 2 * kWave + i % 2 * 16) * 16) =
+        make_uint2(scaled(ca, as_half2(s[0]), as_half2(m[0])), scaled(cb, as_half2(s[1]), as_half2(m[1])));
   }
 }
 
@@ -188,34 +202,52 @@ struct State {
   bool huge;
 };
 
+// Attends two pages, the first one's tokens from position pos on.
 template <int D>
-__device__ inline void attend(const Page<D>& page, int valid, int pos, int lane, State<D>& st) {
+__device__ inline void attend(const Page<D> (&page)[2], int pos, int lane, State<D>& st) {
+  constexpr int kNG = Format<D>::NG, kNC = Format<D>::NC, kOps = D / 16;
   const int h = lane / 32;
+  // each page's valid tokens (lane 2 NG) and NaN words (lanes before it)
+  const int at = min(lane, 2 * kNG);
+  const uint32_t info0 = (&page[0].nan[0][0])[at], info1 = (&page[1].nan[0][0])[at];
   // The operands are read ahead of the products that take them, the values'
-  // before the exponentials: read one by one, the LDS's latency took more
-  // than half of the time.
-  half8 op[D / 16];
+  // before the exponentials: read one by one, the LDS's latency took half of
+  // the time.
+  half8 op[kOps];
+  f32x16 z[2];
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) op[i] = page.k[i][lane];
+  for (int i = 0; i < kOps; ++i) op[i] = page[0].k[i][lane];
   __builtin_amdgcn_sched_barrier(0);
-  f32x16 z{};
+  z[0] = f32x16{};
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) z = mfma32(op[i], st.q[i], z);
+  for (int i = 0; i < kOps; ++i) z[0] = mfma32(op[i], st.q[i], z[0]);
+#pragma unroll
+  for (int i = 0; i < kOps; ++i) op[i] = page[1].k[i][lane];
   __builtin_amdgcn_sched_barrier(0);
+  z[1] = f32x16{};
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) op[i] = page.v[i / 2][i % 2][lane];
+  for (int i = 0; i < kOps; ++i) z[1] = mfma32(op[i], st.q[i], z[1]);
+#pragma unroll
+  for (int i = 0; i < kOps; ++i) op[i] = page[0].v[i / 2][i % 2][lane];
   __builtin_amdgcn_sched_barrier(0);
-  const bool cut = st.first - pos < kPageTokens - 1;  // some row does not see all of the page
-  int seen = valid;
-  if (cut || valid < kPageTokens) {
-    seen = min(seen, max(st.limit - pos + 1, 0));
+
+  const int valid0 = __builtin_amdgcn_readlane(info0, 2 * kNG), valid1 = __builtin_amdgcn_readlane(info1, 2 * kNG);
+  // some row does not see all of the two pages
+  const bool cut = st.first - pos < 2 * kPageTokens - 1 || valid0 < kPageTokens || valid1 < kPageTokens;
+  const int left = max(st.limit - pos + 1, 0);
+  const int seen[2] = {min(valid0, left), min(valid1, max(left - kPageTokens, 0))};
+  const int sees[2] = {seen[0] - 4 * h, seen[1] - 4 * h};  // of the lane's tokens 8 (i / 4) + i % 4
+  if (cut) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) z[i] = 8 * (i / 4) + 4 * h + i % 4 < seen ? z[i] : kLowest;
+    for (int i = 0; i < 32; ++i) z[i / 16][i % 16] = 8 * (i % 16 / 4) + i % 4 < sees[i / 16] ? z[i / 16][i % 16] : kLowest;
   }
-  float top = z[0];
+  float tops[2] = {z[0][0], z[1][0]};
 #pragma unroll
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, z[i]);
-  top *= st.factor;
+  for (int i = 1; i < 16; ++i) {
+    tops[0] = fmaxf(tops[0], z[0][i]);
+    tops[1] = fmaxf(tops[1], z[1][i]);
+  }
+  float top = fmaxf(tops[0], tops[1]) * st.factor;
   if (__any(top > st.m + kLag)) {
     top = fmaxf(xor_max<32>(top), st.m);
     const float f = top > st.m ? __builtin_amdgcn_exp2f(st.m - top) : 1.0f;
@@ -226,40 +258,57 @@ __device__ inline void attend(const Page<D>& page, int valid, int pos, int lane,
     for (int c = 0; c < D / 32; ++c) st.acc[c] *= f;
   }
   const float off = kShift - st.m;
+  if (__builtin_expect(st.huge, false)) {
+    asm volatile("");  // a branch: as a select it would cost three instructions a score
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    float x = __builtin_fmaf(z[i], st.factor, off);
-    if (st.huge) x = z[i] * st.factor + off;
-    z[i] = __builtin_amdgcn_exp2f(x);
+    for (int i = 0; i < 32; ++i) z[i / 16][i % 16] = z[i / 16][i % 16] * st.factor + off;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) z[i / 16][i % 16] = __builtin_fmaf(z[i / 16][i % 16], st.factor, off);
   }
-  if (cut || valid < kPageTokens) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) z[i] = 8 * (i / 4) + 4 * h + i % 4 < seen ? z[i] : 0.0f;
+  for (int i = 0; i < 32; ++i) z[i / 16][i % 16] = __builtin_amdgcn_exp2f(z[i / 16][i % 16]);
+  if (cut) {
+    int again[2] = {sees[0], sees[1]};
+    asm volatile("" : "+v"(again[0]), "+v"(again[1]));  // 32 comparisons kept from above would not fit the registers
+#pragma unroll
+    for (int i = 0; i < 32; ++i) z[i / 16][i % 16] = 8 * (i % 16 / 4) + i % 4 < again[i / 16] ? z[i / 16][i % 16] : 0.0f;
   }
   // the denominator adds what the numerator multiplies: the rounded ones
-  uint32_t pairs[8];
+  uint32_t pairs[16];
+  float sum[2] = {st.l, 0.0f};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const half2_t pair = __builtin_convertvector(float2_t{z[2 * i], z[2 * i + 1]}, half2_t);
-    st.l = __builtin_amdgcn_fdot2(pair, half2_t{1, 1}, st.l, false);
+  for (int i = 0; i < 16; ++i) {
+    const half2_t pair = __builtin_convertvector(float2_t{z[i / 8][2 * i % 16], z[i / 8][2 * i % 16 + 1]}, half2_t);
+    sum[i % 2] = __builtin_amdgcn_fdot2(pair, half2_t{1, 1}, sum[i % 2], false);
     pairs[i] = bits_of(pair);
   }
-  const half8 p0 = as_half8(pairs[0], pairs[1], pairs[2], pairs[3]);
-  const half8 p1 = as_half8(pairs[4], pairs[5], pairs[6], pairs[7]);
+  st.l = sum[0] + sum[1];
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) {
-    st.acc[c] = mfma32(op[2 * c], p0, st.acc[c]);
-    st.acc[c] = mfma32(op[2 * c + 1], p1, st.acc[c]);
+  for (int s = 0; s < 2; ++s) {
+    const half8 p0 = as_half8(pairs[8 * s], pairs[8 * s + 1], pairs[8 * s + 2], pairs[8 * s + 3]);
+    const half8 p1 = as_half8(pairs[8 * s + 4], pairs[8 * s + 5], pairs[8 * s + 6], pairs[8 * s + 7]);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) st.acc[c] = mfma32(op[2 * c], p0, st.acc[c]);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) st.acc[c] = mfma32(op[2 * c + 1], p1, st.acc[c]);
+    if (s == 0) {
+#pragma unroll
+      for (int i = 0; i < kOps; ++i) op[i] = page[1].v[i / 2][i % 2][lane];
+    }
   }
-  constexpr int kNG = Format<D>::NG, kNC = Format<D>::NC;
-  if (__any(lane < 2 * kNG && page.nan[lane / kNG % 2][lane % kNG] != 0)) {
-    const uint32_t sees = seen >= 32 ? ~0u : (1u << seen) - 1u;
+  if (__builtin_expect(__any(lane < 2 * kNG && (info0 | info1) != 0), false)) {
+    asm volatile("");
+#pragma unroll 1
+    for (int s = 0; s < 2; ++s) {
+      const uint32_t visible = seen[s] >= 32 ? ~0u : (1u << seen[s]) - 1u;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {  // channel NC (8 (i / 4) + 4 h + i % 4) + .. of rows 0..15, and again 16..31
-      const int g = (8 * (i / 4 % 2) + 4 * h + i % 4) * kNC / 32;
-      if ((page.nan[0][g] | page.nan[1][g] << 16) & sees) {
+      for (int i = 0; i < 16; ++i) {  // channel NC (8 (i / 4) + 4 h + i % 4) + .. of rows 0..15, and again 16..31
+        const int g = (8 * (i / 4 % 2) + 4 * h + i % 4) * kNC / 32;
+        if ((page[s].nan[0][g] | page[s].nan[1][g] << 16) & visible) {
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) st.acc[c][i] = __builtin_nanf("");
+          for (int c = 0; c < D / 32; ++c) st.acc[c][i] = __builtin_nanf("");
+        }
       }
     }
   }
@@ -299,6 +348,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int h = lane / 32;
+  const Place<D> place(wave, lane);
   const int64_t w = blockIdx.x;
   const int64_t per_head = p.tile_info[1];
   const int tiles = static_cast<int>(p.tile_info[0]);
@@ -377,40 +427,41 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
     const int64_t page_bytes = static_cast<int64_t>(p.kv_heads) * F::kRecord;
     const uint8_t* pool = p.pool + static_cast<int64_t>(head) * F::kRecord;
     PageRef ref{0, 0};
-    int looked = p0 - kWave;  // the lanes hold pages [looked, looked + 64)
-    Raw<D> raw;
-    const auto get = [&](int i) {  // page i into registers; its valid tokens
-      if (i - looked >= kWave) {
+    int looked = p0 - 2 * kWave;  // the lanes hold pages [looked, looked + 64)
+    Raw<D> raw[2];
+    int raw_valid[2];
+    const auto get = [&](int i) {  // pages i and i + 1 into registers (the second may not be there)
+      if (i + 1 - looked >= kWave) {
         looked = i;
         ref = PageRef{0, 0};
         if (i + lane < p1) ref = resolve(p, b, L, i + lane);
       }
-      const int64_t page = __builtin_amdgcn_readlane(ref.page, i - looked);
-      fetch<D>(pool + page * page_bytes, wave, lane, raw);
-      return __builtin_amdgcn_readlane(ref.valid, i - looked);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int64_t page = __builtin_amdgcn_readlane(ref.page, i + s - looked);
+        fetch<D>(pool + page * page_bytes, place, wave, raw[s]);
+        raw_valid[s] = __builtin_amdgcn_readlane(ref.valid, i + s - looked);
+      }
     };
-    int raw_valid = get(p0);
-    const auto put = [&](int i, Page<D>& page) {  // page i, which is in registers; then the next one into them
-      convert<D>(raw, page, raw_valid, wave, lane);
-      if (i + 1 < p1) raw_valid = get(i + 1);
+    const auto put = [&](int i, Page<D>* page) {  // pages i and i + 1, which are in registers; then the next two into them
+#pragma unroll
+      for (int s = 0; s < 2; ++s) convert<D>(raw[s], page[s], raw_valid[s], place, wave, lane);
+      if (i + 2 < p1) get(i + 2);
     };
-    const auto use = [&](int i, const Page<D>& page) {
-      const int pos = i * kPageTokens;
-      if (pos > st.last) return;
-      const int valid = __builtin_amdgcn_readfirstlane(page.valid);
-      if (valid > 0) attend<D>(page, valid, pos, lane, st);
-    };
-    // [a, z) are attended out of one set while [z, y) go into the other; sets
-    // grow from one page, so that the first is not waited for longer.  (One
-    // place in the code for each: two would copy the sums between them.)
-    put(p0, s_page[0][0]);
+    // Pages [a, z) are attended out of one set while [z, y) go into the other,
+    // in pairs; sets grow from one pair, so that the first is not waited for
+    // longer.  (One place in the code for each: two would copy the sums
+    // between them.)
+    get(p0);
+    put(p0, s_page[0]);
     lds_barrier();
-    const int late = wave / (kWaves / 2);
-    for (int a = p0, z = p0 + 1, set = 0; a < p1; set ^= 1) {
-      const int y = min(p1, z + min(kBatch, 2 * (z - a)));
-      for (int i = 0; i < max(z - a, y - z) + late; ++i) {
-        if (i >= late && z + i - late < y) put(z + i - late, s_page[set ^ 1][i - late]);
-        if (a + i < z) use(a + i, s_page[set][i]);
+    const int late = wave / (kWaves / 2) * 2;
+    for (int a = p0, z = p0 + 2, set = 0; a < p1; set ^= 1) {
+      const int y = min((p1 - p0 + 1) / 2 * 2 + p0, z + min(kBatch, 2 * (z - a)));
+      for (int i = 0; i < max(z - a, y - z) + late; i += 2) {
+        if (i >= late && z + i - late < y) put(z + i - late, s_page[set ^ 1] + (i - late));
+        if (a + i < z && (a + i) * kPageTokens <= st.last)
+          attend<D>(*reinterpret_cast<const Page<D>(*)[2]>(s_page[set] + i), (a + i) * kPageTokens, lane, st);
       }
       lds_barrier();
       a = z;
