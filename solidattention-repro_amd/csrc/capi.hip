@@ -1655,6 +1655,10 @@ int sa_hip_kv4_decode_attention(const sa_paged_kv* kv, const void* query, int32_
       return fail(SA_HIP_EINVAL, "%s: select_groups must divide kv_heads", op);
     if (sel_stride <= 0) return fail(SA_HIP_EINVAL, "%s: sel_stride must be positive", op);
   }
+  const int64_t pages = static_cast<int64_t>(kv->table_stride) + (selected ? sel_stride : 0) + 1;
+  if (pages * kv->batch * kv->kv_heads >= (1LL << 31))
+    return fail(SA_HIP_EINVAL, "%s: %d sequences x %d heads x %lld pages exceed 2^31 page reads a call", op, kv->batch,
+                kv->kv_heads, static_cast<long long>(pages));
   sa::Kv4AttnLaunch a{};
   if (int e = kv4_attention(kv, query, type, q_stride, kv->batch, scale, out, workspace, workspace_bytes, status, op, &a))
     return e;

@@ -27,6 +27,7 @@
 #include "kv4_attention.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace sa {
 namespace {
@@ -141,12 +142,12 @@ struct Rows {
   half8 lo[RT][kFine ? F::NG : 1];
   half8 sums[RT];         // operand of the minima
   float factor[RT];
-  int64_t limit[RT];      // last position the row sees
+  int limit[RT];          // last position the row sees
 };
 
 template <int D, int RT, bool kFine>
 __device__ inline void load_rows(const Params& p, Rows<D, RT, kFine>& q, int64_t token0, int n_tokens, int head0,
-                                 int row0, int64_t limit0, int lane) {
+                                 int row0, int limit0, int lane) {
   using F = Format<D>;
   const int r = lane % 16, j = lane / 16;
 #pragma unroll
@@ -255,11 +256,11 @@ __device__ inline void add_values(const Record<D>& x, const half8 (&ph)[RT], con
 // Attends one page: `valid` tokens, the first at position pos; kCausal: a
 // row sees the tokens up to its limit.
 template <int D, int RT, bool kFine, bool kCausal>
-__device__ inline void attend(Record<D>& x, int valid, int64_t pos, int64_t first_limit, const Rows<D, RT, kFine>& q,
+__device__ inline void attend(Record<D>& x, int valid, int pos, int first_limit, const Rows<D, RT, kFine>& q,
                               State<D, RT>& st, int lane) {
   using F = Format<D>;
   const int r = lane % 16, j = lane / 16;
-  const bool cut = kCausal && pos + kPageTokens - 1 > first_limit;  // some row does not see all of it
+  const bool cut = kCausal && first_limit - pos < kPageTokens - 1;  // some row does not see all of it
 
   f32x4 z[RT][2];
 #pragma unroll
@@ -302,8 +303,7 @@ __device__ inline void attend(Record<D>& x, int valid, int64_t pos, int64_t firs
     int seen = valid;
     if (masked) {
       if (kCausal) {
-        const int64_t left = q.limit[rt] - pos + 1;
-        if (left < seen) seen = left < 0 ? 0 : static_cast<int>(left);
+        seen = min(seen, max(q.limit[rt] - pos + 1, 0));
       }
 #pragma unroll
       for (int n = 0; n < 8; ++n)
@@ -384,7 +384,7 @@ __device__ inline void attend(Record<D>& x, int valid, int64_t pos, int64_t firs
             if (g < F::NG && (h & 0x7fffu) > 0x7c00u) {
 #pragma unroll
               for (int rt = 0; rt < RT; ++rt)
-                if (pos + t <= q.limit[rt]) st.tail[rt][i] = __builtin_nanf("");
+                if (t <= q.limit[rt] - pos) st.tail[rt][i] = __builtin_nanf("");
             }
           }
         }
@@ -457,82 +457,92 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
   __shared__ float s_m[kWaves][16];
   __shared__ float s_l[kWaves][16];
   __shared__ int s_last;
-  static_assert(sizeof(s_stage) >= (kThreads + 1) * sizeof(int64_t), "the sums over the lists fit a stage");
-  int64_t* s_sum = reinterpret_cast<int64_t*>(&s_stage[0][0]);
   float* s_acc = reinterpret_cast<float*>(&s_stage[0][0]);
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lane = tid % kWave;
   const int r = lane % 16, j = lane / 16;
-  const int64_t w = blockIdx.x;
+  const uint32_t w = blockIdx.x;
 
   // ---- the units of the launch, and where this workgroup's share begins ----
   // A list has at least one unit, so that an empty one is written too.
-  Share sh{0, 0};
-  const int lists = kCausal ? 0 : p.batch * p.select_groups;
-  const int per = (lists + kThreads - 1) / kThreads;
+  using unit_t = std::conditional_t<kCausal, int64_t, uint32_t>;
+  std::conditional_t<kCausal, Share, SmallShare> sh{};
+  unit_t u, end;
+  unit_t base = 0;  // units before list (decode: the lists of one selection group's heads) or tile s
+  int s = 0;
   if constexpr (kCausal) {
     sh.units = p.tile_info[1] * p.kv_heads;
     if (sh.units <= 0) return;
-  } else {
-    int64_t mine = 0;
-    for (int s = tid * per; s < min((tid + 1) * per, lists); ++s)
-      mine += static_cast<int64_t>(max(decode_list(p, s / p.select_groups, s % p.select_groups).total, 1)) * p.kv_per_sel;
-    int64_t run = mine;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-      const int64_t x = __shfl_up(run, d);
-      if (lane >= d) run += x;
-    }
-    __shared__ int64_t s_wave[kWaves];
-    if (lane == kWave - 1) s_wave[wave] = run;
-    __syncthreads();
-    int64_t before = 0;
-    for (int i = 0; i < kWaves; ++i) {
-      if (i < wave) before += s_wave[i];
-      sh.units += s_wave[i];
-    }
-    s_sum[tid] = before + run - mine;
-    if (tid == 0) s_sum[kThreads] = sh.units;
-    __syncthreads();
-  }
-  sh.groups = min<int64_t>(gridDim.x, max<int64_t>(1, sh.units / kMinUnits));
-  if (w >= sh.groups) return;
-  int64_t u = sh.begin(w);
-  const int64_t end = sh.begin(w + 1);
-
-  // the list (decode: of one selection group's heads) or tile that holds u
-  int64_t base = 0;  // units before it
-  int s = 0;
-  if constexpr (kCausal) {
+    sh.groups = min<int64_t>(gridDim.x, max<int64_t>(1, sh.units / kMinUnits));
+    if (w >= sh.groups) return;
+    u = sh.begin(w);
+    end = sh.begin(w + 1);
     const int64_t at = u % p.tile_info[1];
-    int lo = 0, hi = static_cast<int>(p.tile_info[0]);
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (p.tile_first[mid] <= at) lo = mid;
+    int hi = static_cast<int>(p.tile_info[0]);
+    while (hi - s > 1) {
+      const int mid = (s + hi) / 2;
+      if (p.tile_first[mid] <= at) s = mid;
       else hi = mid;
     }
-    s = lo;
   } else {
-    int lo = 0, hi = kThreads;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (s_sum[mid] <= u) lo = mid;
-      else hi = mid;
+    __shared__ uint32_t s_sum[kWaves], s_first[kWaves], s_found[2];
+    __shared__ int s_even[kWaves];
+    const int lists = p.batch * p.select_groups;
+    const int per = (lists + kThreads - 1) / kThreads;
+    const int first = min(tid * per, lists), last = min(first + per, lists);
+    uint32_t mine = 0, one = 0;  // units of the thread's lists; pages of its first
+    bool even = true;
+    for (int i = first; i < last; ++i) {
+      const uint32_t n = max(decode_list(p, i / p.select_groups, i % p.select_groups).total, 1);
+      if (i == first) one = n;
+      even = even && n == one;
+      mine += n * p.kv_per_sel;
     }
-    s = lo * per;
-    base = s_sum[lo];
-    __syncthreads();  // the sums are read: records may be fetched over them
+    const uint32_t run = wave_prefix_sum(mine);
+    const uint32_t head = __builtin_amdgcn_readfirstlane(one);
+    even = __all(even && (first == last || one == head));
+    if (lane == kWave - 1) {
+      s_sum[wave] = run;
+      s_first[wave] = head;
+      s_even[wave] = even;
+    }
+    __syncthreads();
+    uint32_t before = 0;
+    bool alike = true;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      if (i < wave) before += s_sum[i];
+      sh.units += s_sum[i];
+      alike = alike && s_even[i] && (s_first[i] == s_first[0] || s_sum[i] == 0);
+    }
+    sh.groups = min(gridDim.x, max(1u, sh.units / kMinUnits));
+    // Lists of one length are cut into as many shares each, so that no share
+    // crosses from one into the next: one that does writes its sums twice.
+    const uint32_t all = static_cast<uint32_t>(lists) * p.kv_per_sel;
+    if (alike && all <= gridDim.x) sh.groups = all * max(1u, sh.groups / all);
+    if (w >= sh.groups) return;
+    sh.divide();
+    u = sh.begin(w);
+    end = sh.begin(w + 1);
+    before += run - mine;
+    if (u - before < mine) {  // (u < before wraps to more than any)
+      s_found[0] = first;
+      s_found[1] = before;
+    }
+    __syncthreads();
+    s = __builtin_amdgcn_readfirstlane(s_found[0]);
+    base = __builtin_amdgcn_readfirstlane(s_found[1]);
   }
 
   while (u < end) {
     // ---- the list, its rows, and this share's pages [p0, p1) of it ----
     int b, h;
     List L;
-    int64_t list_first;  // unit of the list's first page
+    unit_t list_first;   // unit of the list's first page
     int pages;           // units of the list
     Target tg;
-    int64_t limit0 = 0;
+    int limit0 = 0;
     if constexpr (kCausal) {
       const int64_t per_head = p.tile_info[1];
       h = static_cast<int>(u / per_head);
@@ -544,18 +554,18 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
       tg.n_tokens = p.query_start[b + 1] - p.query_start[b];
       tg.row0 = t.y;
       const int64_t len = p.seq_len[b];
-      limit0 = len - tg.n_tokens;
+      limit0 = static_cast<int>(len) - tg.n_tokens;
       L = List{nullptr, len, 0, 0, static_cast<int>((len + kPageTokens - 1) / kPageTokens)};
     } else {
       for (;;) {
         b = s / p.select_groups;
         L = decode_list(p, b, s % p.select_groups);
         pages = max(L.total, 1);
-        if (u < base + static_cast<int64_t>(pages) * p.kv_per_sel) break;
-        base += static_cast<int64_t>(pages) * p.kv_per_sel;
+        if (u < base + static_cast<unit_t>(pages) * p.kv_per_sel) break;
+        base += static_cast<unit_t>(pages) * p.kv_per_sel;
         ++s;
       }
-      const int64_t k = (u - base) / pages;
+      const unit_t k = (u - base) / pages;
       h = (s % p.select_groups) * p.kv_per_sel + static_cast<int>(k);
       list_first = base + k * pages;
       tg.token0 = b;
@@ -564,28 +574,32 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
     }
     tg.head0 = h * p.group;
     const int p0 = static_cast<int>(u - list_first);
-    const int p1 = static_cast<int>(min<int64_t>(pages, p0 + (end - u)));
+    const int p1 = static_cast<int>(min<int64_t>(pages, p0 + static_cast<int64_t>(end - u)));
 
+    // A lane looks up one of the wave's next 64 pages, so that the chain
+    // selected id -> table -> record is walked once for all of them, and the
+    // first record is on its way while the rows are read.
+    const int64_t head_off = static_cast<int64_t>(h) * F::kRecord;
+    const int64_t page_bytes = static_cast<int64_t>(p.kv_heads) * F::kRecord;
+    PageRef ref{0, 0};
+    const auto fetch = [&](int k) {
+      const int64_t page = __builtin_amdgcn_readlane(ref.page, k);
+      fetch_record<D>(p.pool + (page * page_bytes + head_off), s_stage[wave], lane);
+    };
+    const auto look = [&](int at) {
+      ref = PageRef{0, 0};
+      if (at + kWaves * lane < p1) ref = resolve(p, b, L, at + kWaves * lane);
+      if (at < p1) fetch(0);
+    };
+    int at = p0 + wave;
+    look(at);
     Rows<D, RT, kFine> q;
     load_rows<D, RT, kFine>(p, q, tg.token0, tg.n_tokens, tg.head0, tg.row0, limit0, lane);
     State<D, RT> st;
     st.reset();
-    const int64_t first_limit = limit0 + tg.row0 / p.group;
-    const int64_t head_off = static_cast<int64_t>(h) * F::kRecord;
-    const int64_t page_bytes = static_cast<int64_t>(p.kv_heads) * F::kRecord;
-
-    // A lane looks up one of the wave's next 64 pages, so that the chain
-    // selected id -> table -> record is walked once for all of them.
-    for (int at = p0 + wave; at < p1; at += kWaves * kWave) {
-      const int mine = at + kWaves * lane;
-      PageRef ref{0, 0};
-      if (mine < p1) ref = resolve(p, b, L, mine);
+    const int first_limit = limit0 + tg.row0 / p.group;
+    while (at < p1) {
       const int n = min(kWave, (p1 - at + kWaves - 1) / kWaves);
-      const auto fetch = [&](int k) {
-        const int64_t page = __builtin_amdgcn_readlane(ref.page, k);
-        fetch_record<D>(p.pool + (page * page_bytes + head_off), s_stage[wave], lane);
-      };
-      fetch(0);
       for (int k = 0; k < n; ++k) {
         wait_fetch();
         Record<D> x;
@@ -594,14 +608,14 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
         if (k + 1 < n) fetch(k + 1);
         const int valid = __builtin_amdgcn_readlane(ref.valid, k);
         if (valid > 0)
-          attend<D, RT, kFine, kCausal>(x, valid, static_cast<int64_t>(at + kWaves * k) * kPageTokens, first_limit, q, st,
-                                        lane);
+          attend<D, RT, kFine, kCausal>(x, valid, (at + kWaves * k) * kPageTokens, first_limit, q, st, lane);
       }
+      at += kWaves * kWave;
+      if (at < p1) look(at);
     }
 
     // ---- the waves' states, then the shares' records ----
     const bool whole = p0 == 0 && p1 == pages;
-    const int64_t w0 = sh.owner(list_first), w1 = sh.owner(list_first + pages - 1);
     float* rec = p.records + (2 * w + (p0 == 0 ? 1 : 0)) * static_cast<int64_t>(kRecFloats);
     const int live_rows = min(kRows, tg.n_tokens * p.group - tg.row0);
 #pragma unroll
@@ -662,26 +676,77 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
         }
       }
     }
-    if (!whole && last_arrival(p.arrive + w0, static_cast<int>(w1 - w0 + 1), &s_last)) {
+    if (!whole) {
+      const uint32_t w0 = sh.owner(list_first), w1 = sh.owner(list_first + pages - 1);
       const int shares = static_cast<int>(w1 - w0 + 1);
-      const float* first = p.records + (2 * w0 + 1) * static_cast<int64_t>(kRecFloats);
-      const auto record = [&](int i) { return i == 0 ? first : p.records + 2 * (w0 + i) * static_cast<int64_t>(kRecFloats); };
-      for (int e = tid; e < live_rows * (D / 4); e += kThreads) {
-        const int row = e / (D / 4), ch = e % (D / 4) * 4;
-        float top = kNegInf;
-        for (int i = 0; i < shares; ++i) top = fmaxf(top, load_agent(record(i) + 2 * row));
-        float sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i = 0; i < shares; ++i) {
-          const float* y = record(i);
-          const float m = load_agent(y + 2 * row), l = load_agent(y + 2 * row + 1);
-          const float f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-          sum = __builtin_fmaf(l, f, sum);
+      if (last_arrival(p.arrive + w0, shares, &s_last)) {
+        const auto record = [&](int i) {
+          return p.records + (2 * static_cast<int64_t>(w0 + i) + (i == 0 ? 1 : 0)) * kRecFloats;
+        };
+        // Four channels a thread; with threads to spare each takes every
+        // `parts`-th record, and the parts meet in LDS, in order.
+        const int quads = live_rows * (D / 4);
+        const int parts = min(max(kThreads / quads, 1), shares);
+        const int part = tid / quads;
+        for (int e0 = 0; e0 < quads; e0 += kThreads) {
+          const int e = parts > 1 ? tid - part * quads : e0 + tid;
+          const bool on = parts > 1 ? part < parts : e < quads;
+          const int row = e / (D / 4), ch = e % (D / 4) * 4;
+          // In 64 bits: a share of small weights added to one of a large one
+          // loses the same bits every time.
+          float top = kNegInf;
+          double sum = 0.0, x[4] = {0.0, 0.0, 0.0, 0.0};
+          const auto add = [&](float m, float l, const float* y) {
+            const float to = fmaxf(top, m);
+            const double f = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+            const double g = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+            top = to;
+            sum = __builtin_fma(l, f, sum * g);
 #pragma unroll
-          for (int n = 0; n < 4; ++n) x[n] = __builtin_fmaf(load_agent(y + 2 * kRows + row * D + ch + n), f, x[n]);
+            for (int n = 0; n < 4; ++n) x[n] = __builtin_fma(y[n], f, x[n] * g);
+          };
+          if (on) {
+            constexpr int kAtOnce = 4;  // loads in flight
+            const int from = parts > 1 ? part : 0;
+            for (int i = from; i < shares; i += parts * kAtOnce) {
+              float m[kAtOnce], l[kAtOnce], y[kAtOnce][4];
+#pragma unroll
+              for (int a = 0; a < kAtOnce; ++a) {
+                const float* z = record(min(i + a * parts, shares - 1));
+                m[a] = load_agent(z + 2 * row);
+                l[a] = load_agent(z + 2 * row + 1);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) y[a][n] = load_agent(z + 2 * kRows + row * D + ch + n);
+              }
+#pragma unroll
+              for (int a = 0; a < kAtOnce; ++a) {
+                if (i + a * parts < shares) add(m[a], l[a], y[a]);
+              }
+            }
+          }
+          if (parts > 1) {
+            float* to = s_acc + (part * quads + e) * 6;
+            if (on) {
+              to[0] = top;
+              to[1] = static_cast<float>(sum);
+#pragma unroll
+              for (int n = 0; n < 4; ++n) to[2 + n] = static_cast<float>(x[n]);
+            }
+            __syncthreads();
+            if (part == 0) {
+              for (int a = 1; a < parts; ++a) {
+                const float* z = s_acc + (a * quads + e) * 6;
+                add(z[0], z[1], z + 2);
+              }
+            }
+          }
+          if (on && (parts == 1 || part == 0)) {
+            float y[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) y[n] = sum == 0.0 ? 0.0f : static_cast<float>(x[n]) / static_cast<float>(sum);
+            store_out(p, tg.token0 + (tg.row0 + row) / p.group, tg.head0 + (tg.row0 + row) % p.group, D, ch, y);
+          }
         }
-#pragma unroll
-        for (int n = 0; n < 4; ++n) x[n] = sum == 0.0f ? 0.0f : x[n] / sum;
-        store_out(p, tg.token0 + (tg.row0 + row) / p.group, tg.head0 + (tg.row0 + row) % p.group, D, ch, x);
       }
     }
 

@@ -174,6 +174,26 @@ struct Share {
   __device__ inline int64_t owner(int64_t u) const { return ((u + 1) * groups - 1) / units; }
 };
 
+// The same in 32 bits, for fewer than 2^31 units and at most 4096 groups: a
+// 64-bit division takes longer than a small list.
+struct SmallShare {
+  uint32_t units;
+  uint32_t groups;
+  uint32_t each, rest;  // units = each * groups + rest
+  __device__ inline void divide() {
+    each = units / groups;
+    rest = units - each * groups;
+  }
+  __device__ inline uint32_t begin(uint32_t w) const { return each * w + rest * w / groups; }
+  __device__ inline uint32_t owner(uint32_t u) const {
+    uint32_t w = static_cast<uint32_t>(static_cast<float>(u) * (static_cast<float>(groups) / static_cast<float>(units)));
+    if (w >= groups) w = groups - 1;
+    while (begin(w) > u) --w;
+    while (begin(w + 1) <= u) ++w;
+    return w;
+  }
+};
+
 struct Target {
   int64_t token0;  // first query row of the sequence
   int n_tokens;
