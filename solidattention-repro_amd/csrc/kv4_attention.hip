@@ -145,56 +145,74 @@ struct Rows {
   int limit[RT];          // last position the row sees
 };
 
+// The workgroup's rows, converted once for its waves: a lane takes 8 channels.
+// (Unrolled for each wave's own operands the conversion was a third of the
+// kernel's code, and fetching instructions took longer than a short list.)
 template <int D, int RT, bool kFine>
-__device__ inline void load_rows(const Params& p, Rows<D, RT, kFine>& q, int64_t token0, int n_tokens, int head0,
-                                 int row0, int limit0, int lane) {
+struct RowStage {
   using F = Format<D>;
+  half8 hi[RT * F::NG][kWave];
+  half8 lo[kFine ? RT * F::NG : 1][kWave];
+  float sum[16 * RT][F::NG];
+  float factor[16 * RT];
+};
+
+template <int D, int RT, bool kFine>
+__device__ inline void load_rows(const Params& p, RowStage<D, RT, kFine>& s, Rows<D, RT, kFine>& q, const Target& tg,
+                                 int limit0) {
+  using F = Format<D>;
+  constexpr int kLanes = D / 8;  // of a row
+  const int tid = threadIdx.x, lane = tid % kWave;
+#pragma unroll 1
+  for (int row = tid / kLanes; row < 16 * RT; row += kThreads / kLanes) {
+    const int c = tid % kLanes, g = c / 4, j = c % 4;
+    const int token = (tg.row0 + row) / p.group;
+    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (token < tg.n_tokens) {
+      const int64_t at = (tg.token0 + token) * p.q_stride +
+                         static_cast<int64_t>(tg.head0 + (tg.row0 + row - token * p.group)) * D + 8 * c;
+      if constexpr (kFine)
+        load8(p.query, at, kF32, x);
+      else
+        load8(p.query, at, p.type == kF16 ? kF16 : kBF16, x);
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) top = fmaxf(top, fabsf(x[n]));
+#pragma unroll
+    for (int n = 1; n < kLanes; n *= 2) top = fmaxf(top, __shfl_xor(top, n));
+    // the row's largest value into [1, 2): a power of two, exact
+    const int e = top > 0.0f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+    half8 hi, lo;
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const int i = n / 2 + (n % 2) * 4;  // operand order (0,4), (1,5), ...
+      const float v = ldexp2(p.qscale < 0.0f ? -x[i] : x[i], -e);
+      hi[n] = static_cast<_Float16>(v);
+      lo[n] = static_cast<_Float16>(v - static_cast<float>(hi[n]));
+      sum += static_cast<float>(hi[n]);
+      if constexpr (kFine) sum += static_cast<float>(lo[n]);
+    }
+    const int slot = (row / 16) * F::NG + g, of = 16 * j + row % 16;
+    s.hi[slot][of] = hi;
+    if constexpr (kFine) s.lo[slot][of] = lo;
+    sum += __shfl_xor(sum, 1);
+    sum += __shfl_xor(sum, 2);
+    if (j == 0) s.sum[row][g] = sum;
+    if (c == 0) s.factor[row] = ldexp2(fabsf(p.qscale), e);  // not negative: the scale's sign goes to q
+  }
+  __syncthreads();
   const int r = lane % 16, j = lane / 16;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int row = row0 + rt * 16 + r;
-    const int token = row / p.group;
-    const bool live = token < n_tokens;
-    q.limit[rt] = live ? limit0 + token : limit0 + (n_tokens - 1);
-    float x[F::NG][8];
-    float top = 0.0f;
+    const int row = rt * 16 + r;
+    q.limit[rt] = limit0 + min((tg.row0 + row) / p.group, tg.n_tokens - 1);
+    q.factor[rt] = s.factor[row];
 #pragma unroll
     for (int g = 0; g < F::NG; ++g) {
-#pragma unroll
-      for (int n = 0; n < 8; ++n) x[g][n] = 0.0f;
-      const int64_t at =
-          (token0 + token) * p.q_stride + static_cast<int64_t>(head0 + row % p.group) * D + 32 * g + 8 * j;
-      if (live) {
-        if constexpr (kFine)
-          load8(p.query, at, kF32, x[g]);
-        else
-          load8(p.query, at, p.type == kF16 ? kF16 : kBF16, x[g]);
-      }
-#pragma unroll
-      for (int n = 0; n < 8; ++n) top = fmaxf(top, fabsf(x[g][n]));
-    }
-    top = xor_max<32>(xor_max<16>(top));
-    // the row's largest value into [1, 2): a power of two, exact
-    const int e = top > 0.0f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
-    q.factor[rt] = ldexp2(fabsf(p.qscale), e);  // not negative: the scale's sign goes to q
-    float sum[F::NG];
-#pragma unroll
-    for (int g = 0; g < F::NG; ++g) {
-      half8 hi, lo;
-      float s = 0.0f;
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const int c = n / 2 + (n % 2) * 4;  // operand order (0,4), (1,5), ...
-        const float v = ldexp2(p.qscale < 0.0f ? -x[g][c] : x[g][c], -e);
-        hi[n] = static_cast<_Float16>(v);
-        lo[n] = static_cast<_Float16>(v - static_cast<float>(hi[n]));
-        s += static_cast<float>(hi[n]);
-        if constexpr (kFine) s += static_cast<float>(lo[n]);
-      }
-      q.hi[rt][g] = hi;
-      if constexpr (kFine) q.lo[rt][g] = lo;
-      s = xor_sum<32>(xor_sum<16>(s));
-      sum[g] = s;
+      q.hi[rt][g] = s.hi[rt * F::NG + g][lane];
+      if constexpr (kFine) q.lo[rt][g] = s.lo[rt * F::NG + g][lane];
     }
     // products of the minima: NG slots of high parts, NG of low ones
     half8 op{};
@@ -203,10 +221,10 @@ __device__ inline void load_rows(const Params& p, Rows<D, RT, kFine>& q, int64_t
       float v = 0.0f;
       bool low = false;
       if constexpr (F::NG == 8) {
-        v = j < 2 ? sum[n] : 0.0f;
+        v = j < 2 ? s.sum[row][n] : 0.0f;
         low = j == 1;
       } else if (n < 2 * F::NG) {
-        v = j == 0 ? sum[n % F::NG] : 0.0f;
+        v = j == 0 ? s.sum[row][n % F::NG] : 0.0f;
         low = n >= F::NG;
       }
       const _Float16 h = static_cast<_Float16>(v);
@@ -417,31 +435,32 @@ __device__ inline float tile_row(const f32x4& t, int row, int lane) {
 constexpr int rows_of(int RT) { return 16 * RT; }
 constexpr size_t record_floats(int D, int rows) { return static_cast<size_t>(rows) * (D + 2); }
 
-// The waves' sums meet in the stage, a chunk of channels at a time.
+// The waves' sums of 16 rows meet where the records were staged, up to 128
+// channels at a time.
 template <int D>
-constexpr int kChunk = D / 32;
-static_assert(kWaves * kChunk<64> * 4 * kWave * sizeof(float) <= kWaves * Format<64>::kRecord, "a chunk fits a stage");
-static_assert(kWaves * kChunk<128> * 4 * kWave * sizeof(float) <= kWaves * Format<128>::kRecord, "a chunk fits a stage");
-static_assert(kWaves * kChunk<256> * 4 * kWave * sizeof(float) <= kWaves * Format<256>::kRecord, "a chunk fits a stage");
+struct Meet {
+  static constexpr int kChannels = D < 128 ? D : 128;
+  static constexpr int kStride = kChannels + 4;  // floats: neighbouring rows in other banks
+  static constexpr int kFloats = 16 * kStride;   // of a wave
+  static constexpr int kBytes = kWaves * kFloats * 4;
+};
 
-template <int N>
-__device__ inline void store_out(const Params& p, int64_t token, int head, int D, int ch, const float (&x)[N]) {
+__device__ inline void store_out2(const Params& p, int64_t token, int head, int D, int ch, float a, float b) {
   const int64_t at = (token * p.query_heads + head) * D + ch;
-  if constexpr (N == 8) {
-    store8(p.out, at, p.type, x);
-  } else if (p.type == kF32) {
-    float* o = static_cast<float*>(p.out) + at;
-    if constexpr (N == 4)
-      *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
-    else
-      *reinterpret_cast<float2*>(o) = make_float2(x[0], x[1]);
-  } else {
-    uint16_t* o = static_cast<uint16_t*>(p.out) + at;
-    if constexpr (N == 4)
-      *reinterpret_cast<uint2*>(o) = make_uint2(pack2(x[0], x[1], p.type), pack2(x[2], x[3], p.type));
-    else
-      *reinterpret_cast<uint32_t*>(o) = pack2(x[0], x[1], p.type);
-  }
+  if (p.type == kF32)
+    *reinterpret_cast<float2*>(static_cast<float*>(p.out) + at) = make_float2(a, b);
+  else
+    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + at) = pack2(a, b, p.type);
+}
+
+// Two floats that another workgroup reads in this launch (8-byte aligned).
+__device__ inline void store_pair(float* at, float a, float b) {
+  store_agent(reinterpret_cast<uint64_t*>(at),
+              static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a));
+}
+__device__ inline float2 load_pair(const float* at) {
+  const uint64_t v = load_agent(reinterpret_cast<const uint64_t*>(at));
+  return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
 }
 
 // Workgroups a compute unit holds, by their registers.
@@ -453,16 +472,20 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
   using F = Format<D>;
   constexpr int kRows = rows_of(RT);
   constexpr int kRecFloats = static_cast<int>(record_floats(D, kRows));
-  __shared__ __align__(16) uint8_t s_stage[kWaves][F::kRecord];
+  using M = Meet<D>;
+  __shared__ __align__(16) uint8_t s_bytes[std::max<int>(kWaves * F::kRecord, M::kBytes)];
+  __shared__ __align__(16) RowStage<D, RT, kFine> s_rows;
   __shared__ float s_m[kWaves][16];
   __shared__ float s_l[kWaves][16];
+  __shared__ float s_sum[16];
   __shared__ int s_last;
-  float* s_acc = reinterpret_cast<float*>(&s_stage[0][0]);
+  float* s_acc = reinterpret_cast<float*>(s_bytes);
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lane = tid % kWave;
   const int r = lane % 16, j = lane / 16;
   const uint32_t w = blockIdx.x;
+  uint8_t* stage = s_bytes + wave * F::kRecord;
 
   // ---- the units of the launch, and where this workgroup's share begins ----
   // A list has at least one unit, so that an empty one is written too.
@@ -486,7 +509,7 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
       else hi = mid;
     }
   } else {
-    __shared__ uint32_t s_sum[kWaves], s_first[kWaves], s_found[2];
+    __shared__ uint32_t s_units[kWaves], s_first[kWaves], s_found[2];
     __shared__ int s_even[kWaves];
     const int lists = p.batch * p.select_groups;
     const int per = (lists + kThreads - 1) / kThreads;
@@ -503,7 +526,7 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
     const uint32_t head = __builtin_amdgcn_readfirstlane(one);
     even = __all(even && (first == last || one == head));
     if (lane == kWave - 1) {
-      s_sum[wave] = run;
+      s_units[wave] = run;
       s_first[wave] = head;
       s_even[wave] = even;
     }
@@ -512,9 +535,9 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
     bool alike = true;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
-      if (i < wave) before += s_sum[i];
-      sh.units += s_sum[i];
-      alike = alike && s_even[i] && (s_first[i] == s_first[0] || s_sum[i] == 0);
+      if (i < wave) before += s_units[i];
+      sh.units += s_units[i];
+      alike = alike && s_even[i] && (s_first[i] == s_first[0] || s_units[i] == 0);
     }
     sh.groups = min(gridDim.x, max(1u, sh.units / kMinUnits));
     // Lists of one length are cut into as many shares each, so that no share
@@ -584,7 +607,7 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
     PageRef ref{0, 0};
     const auto fetch = [&](int k) {
       const int64_t page = __builtin_amdgcn_readlane(ref.page, k);
-      fetch_record<D>(p.pool + (page * page_bytes + head_off), s_stage[wave], lane);
+      fetch_record<D>(p.pool + (page * page_bytes + head_off), stage, lane);
     };
     const auto look = [&](int at) {
       ref = PageRef{0, 0};
@@ -594,7 +617,7 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
     int at = p0 + wave;
     look(at);
     Rows<D, RT, kFine> q;
-    load_rows<D, RT, kFine>(p, q, tg.token0, tg.n_tokens, tg.head0, tg.row0, limit0, lane);
+    load_rows<D, RT, kFine>(p, s_rows, q, tg, limit0);
     State<D, RT> st;
     st.reset();
     const int first_limit = limit0 + tg.row0 / p.group;
@@ -603,7 +626,7 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
       for (int k = 0; k < n; ++k) {
         wait_fetch();
         Record<D> x;
-        read_record<D>(s_stage[wave], lane, x);
+        read_record<D>(stage, lane, x);
         wait_reads();
         if (k + 1 < n) fetch(k + 1);
         const int valid = __builtin_amdgcn_readlane(ref.valid, k);
@@ -641,37 +664,42 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
         if (s_m[i][r] != kNegInf || s_l[i][r] != 0.0f)
           sum = __builtin_fmaf(s_l[i][r], s_m[i][r] == top ? 1.0f : __builtin_amdgcn_exp2f(s_m[i][r] - top), sum);
       const float f = st.m[rt] == top ? 1.0f : __builtin_amdgcn_exp2f(st.m[rt] - top);
-      const int row = rt * 16 + r;
-      const int token = (tg.row0 + row) / p.group, qh = tg.head0 + (tg.row0 + row) % p.group;
-      constexpr int kN = kChunk<D>;
+      const int rows = min(16, live_rows - 16 * rt);
+      if (wave == 0 && j == 0) {
+        s_sum[r] = sum;
+        if (!whole && r < rows) store_pair(rec + 2 * (16 * rt + r), top, sum);
+      }
+      constexpr int kN = M::kChannels / 16;  // of a lane, for each i
 #pragma unroll
       for (int c = 0; c < F::NC / kN; ++c) {
         if (c) __syncthreads();
+        // channel (4j + i) NC + c kN + n stands at (4j + i) kN + n
 #pragma unroll
-        for (int n = 0; n < kN; ++n)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s_acc[((wave * kN + n) * 4 + i) * kWave + lane] = st.acc[rt][c * kN + n][i] * f;
+          for (int n = 0; n < kN; n += 4)
+            *reinterpret_cast<float4*>(s_acc + wave * M::kFloats + r * M::kStride + (4 * j + i) * kN + n) =
+                make_float4(st.acc[rt][c * kN + n][i] * f, st.acc[rt][c * kN + n + 1][i] * f,
+                            st.acc[rt][c * kN + n + 2][i] * f, st.acc[rt][c * kN + n + 3][i] * f);
         __syncthreads();
-        if (row < live_rows) {  // wave i adds up channels (4j + i) NC ..
-          float x[kN];
+#pragma unroll 1
+        for (int e = tid; e < rows * (M::kChannels / 2); e += kThreads) {
+          const int of = e / (M::kChannels / 2), at = e % (M::kChannels / 2) * 2;
+          const int row = 16 * rt + of, ch = at / kN * F::NC + c * kN + at % kN;
+          float a = 0.0f, b = 0.0f;
 #pragma unroll
-          for (int n = 0; n < kN; ++n) {
-            x[n] = 0.0f;
-#pragma unroll
-            for (int v = 0; v < kWaves; ++v) x[n] += s_acc[((v * kN + n) * 4 + wave) * kWave + lane];
+          for (int v = 0; v < kWaves; ++v) {
+            const float2 y = *reinterpret_cast<const float2*>(s_acc + v * M::kFloats + of * M::kStride + at);
+            a += y.x;
+            b += y.y;
           }
-          const int ch = (4 * j + wave) * F::NC + c * kN;
           if (whole) {
-#pragma unroll
-            for (int n = 0; n < kN; ++n) x[n] = sum == 0.0f ? 0.0f : x[n] / sum;
-            store_out(p, tg.token0 + token, qh, D, ch, x);
+            const float l = s_sum[of];
+            const int token = (tg.row0 + row) / p.group;
+            store_out2(p, tg.token0 + token, tg.head0 + (tg.row0 + row - token * p.group), D, ch,
+                       l == 0.0f ? 0.0f : a / l, l == 0.0f ? 0.0f : b / l);
           } else {
-#pragma unroll
-            for (int n = 0; n < kN; ++n) store_agent(rec + 2 * kRows + row * D + ch + n, x[n]);
-            if (c == 0 && wave == 0 && j == 0) {
-              store_agent(rec + 2 * row, top);
-              store_agent(rec + 2 * row + 1, sum);
-            }
+            store_pair(rec + 2 * kRows + row * D + ch, a, b);
           }
         }
       }
@@ -683,69 +711,58 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
         const auto record = [&](int i) {
           return p.records + (2 * static_cast<int64_t>(w0 + i) + (i == 0 ? 1 : 0)) * kRecFloats;
         };
-        // Four channels a thread; with threads to spare each takes every
+        // Two channels a thread; with threads to spare each takes every
         // `parts`-th record, and the parts meet in LDS, in order.
-        const int quads = live_rows * (D / 4);
-        const int parts = min(max(kThreads / quads, 1), shares);
-        const int part = tid / quads;
-        for (int e0 = 0; e0 < quads; e0 += kThreads) {
-          const int e = parts > 1 ? tid - part * quads : e0 + tid;
-          const bool on = parts > 1 ? part < parts : e < quads;
-          const int row = e / (D / 4), ch = e % (D / 4) * 4;
+        const int pairs = live_rows * (D / 2);
+        const int parts = min(max(kThreads / pairs, 1), shares);
+        const int part = parts > 1 ? tid / pairs : 0;
+#pragma unroll 1
+        for (int e = tid - part * pairs; e < pairs; e += kThreads) {
+          const int row = e / (D / 2), ch = e % (D / 2) * 2;
           // In 64 bits: a share of small weights added to one of a large one
           // loses the same bits every time.
           float top = kNegInf;
-          double sum = 0.0, x[4] = {0.0, 0.0, 0.0, 0.0};
-          const auto add = [&](float m, float l, const float* y) {
+          double sum = 0.0, a = 0.0, b = 0.0;
+          const auto add = [&](float m, float l, float x, float y) {
             const float to = fmaxf(top, m);
             const double f = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
             const double g = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
             top = to;
             sum = __builtin_fma(l, f, sum * g);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) x[n] = __builtin_fma(y[n], f, x[n] * g);
+            a = __builtin_fma(x, f, a * g);
+            b = __builtin_fma(y, f, b * g);
           };
-          if (on) {
-            constexpr int kAtOnce = 4;  // loads in flight
-            const int from = parts > 1 ? part : 0;
-            for (int i = from; i < shares; i += parts * kAtOnce) {
-              float m[kAtOnce], l[kAtOnce], y[kAtOnce][4];
+          constexpr int kAtOnce = 8;  // records on their way
+#pragma unroll 1
+          for (int i = part; part < parts && i < shares; i += parts * kAtOnce) {
+            float2 ml[kAtOnce], x[kAtOnce];
 #pragma unroll
-              for (int a = 0; a < kAtOnce; ++a) {
-                const float* z = record(min(i + a * parts, shares - 1));
-                m[a] = load_agent(z + 2 * row);
-                l[a] = load_agent(z + 2 * row + 1);
-#pragma unroll
-                for (int n = 0; n < 4; ++n) y[a][n] = load_agent(z + 2 * kRows + row * D + ch + n);
-              }
-#pragma unroll
-              for (int a = 0; a < kAtOnce; ++a) {
-                if (i + a * parts < shares) add(m[a], l[a], y[a]);
-              }
+            for (int n = 0; n < kAtOnce; ++n) {
+              const float* z = record(min(i + n * parts, shares - 1));
+              ml[n] = load_pair(z + 2 * row);
+              x[n] = load_pair(z + 2 * kRows + row * D + ch);
             }
+#pragma unroll
+            for (int n = 0; n < kAtOnce; ++n)
+              if (i + n * parts < shares) add(ml[n].x, ml[n].y, x[n].x, x[n].y);
           }
-          if (parts > 1) {
-            float* to = s_acc + (part * quads + e) * 6;
-            if (on) {
-              to[0] = top;
-              to[1] = static_cast<float>(sum);
-#pragma unroll
-              for (int n = 0; n < 4; ++n) to[2 + n] = static_cast<float>(x[n]);
-            }
+          if (parts > 1) {  // (one round of the loop)
+            float* to = s_acc + (part * pairs + e) * 4;
+            to[0] = top;
+            to[1] = static_cast<float>(sum);
+            to[2] = static_cast<float>(a);
+            to[3] = static_cast<float>(b);
             __syncthreads();
-            if (part == 0) {
-              for (int a = 1; a < parts; ++a) {
-                const float* z = s_acc + (a * quads + e) * 6;
-                add(z[0], z[1], z + 2);
-              }
+            if (part > 0) break;
+            for (int n = 1; n < parts; ++n) {
+              const float* z = s_acc + (n * pairs + e) * 4;
+              add(z[0], z[1], z[2], z[3]);
             }
           }
-          if (on && (parts == 1 || part == 0)) {
-            float y[4];
-#pragma unroll
-            for (int n = 0; n < 4; ++n) y[n] = sum == 0.0 ? 0.0f : static_cast<float>(x[n]) / static_cast<float>(sum);
-            store_out(p, tg.token0 + (tg.row0 + row) / p.group, tg.head0 + (tg.row0 + row) % p.group, D, ch, y);
-          }
+          const float l = static_cast<float>(sum);
+          const int token = (tg.row0 + row) / p.group;
+          store_out2(p, tg.token0 + token, tg.head0 + (tg.row0 + row - token * p.group), D, ch,
+                     sum == 0.0 ? 0.0f : static_cast<float>(a) / l, sum == 0.0 ? 0.0f : static_cast<float>(b) / l);
         }
       }
     }
