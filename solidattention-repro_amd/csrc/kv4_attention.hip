@@ -63,8 +63,9 @@ __device__ inline void fetch_record(const uint8_t* rec, uint8_t* slot, int lane)
       __builtin_amdgcn_global_load_lds((GlobalPtr)(rec + at + lane * 16), (LdsPtr)(slot + at), 16, 0, kDmaNontemporal);
 }
 __device__ inline void wait_fetch() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-// The slot may be fetched into once its reads have returned.
-__device__ inline void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// The slot may be fetched into once its reads have returned; another lane's
+// word may be read once it has been written.
+__device__ inline void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 template <int D>
 struct Record {
@@ -418,18 +419,6 @@ __device__ inline void attend(Record<D>& x, int valid, int pos, int first_limit,
   add_values<D, RT, 0>(x, ph, pl, kFine, st);
 }
 
-// Component `row` (0..15) of this lane's column of a 16x16 tile.
-__device__ inline float tile_row(const f32x4& t, int row, int lane) {
-  const int from = (row / 4) * 16 + lane % 16;
-  float v = 0.0f;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const float x = __shfl(t[c], from);
-    if (row % 4 == c) v = x;
-  }
-  return v;
-}
-
 // ---- shares of the row of units ---------------------------------------------------
 
 constexpr int rows_of(int RT) { return 16 * RT; }
@@ -478,6 +467,7 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
   __shared__ float s_m[kWaves][16];
   __shared__ float s_l[kWaves][16];
   __shared__ float s_sum[16];
+  __shared__ __align__(16) float s_tail[kWaves][16][20];
   __shared__ int s_last;
   float* s_acc = reinterpret_cast<float*>(s_bytes);
   const int tid = threadIdx.x;
@@ -495,19 +485,11 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
   unit_t base = 0;  // units before list (decode: the lists of one selection group's heads) or tile s
   int s = 0;
   if constexpr (kCausal) {
-    sh.units = p.tile_info[1] * p.kv_heads;
-    if (sh.units <= 0) return;
-    sh.groups = min<int64_t>(gridDim.x, max<int64_t>(1, sh.units / kMinUnits));
-    if (w >= sh.groups) return;
-    u = sh.begin(w);
-    end = sh.begin(w + 1);
-    const int64_t at = u % p.tile_info[1];
-    int hi = static_cast<int>(p.tile_info[0]);
-    while (hi - s > 1) {
-      const int mid = (s + hi) / 2;
-      if (p.tile_first[mid] <= at) s = mid;
-      else hi = mid;
-    }
+    const Start at = start_share(p, sh, w, kMinUnits, lane);
+    if (!at.any) return;
+    s = at.s;
+    u = at.u;
+    end = at.end;
   } else {
     __shared__ uint32_t s_units[kWaves], s_first[kWaves], s_found[2];
     __shared__ int s_even[kWaves];
@@ -515,34 +497,45 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
     const int per = (lists + kThreads - 1) / kThreads;
     const int first = min(tid * per, lists), last = min(first + per, lists);
     uint32_t mine = 0, one = 0;  // units of the thread's lists; pages of its first
+    uint32_t most = 0;           // and of its longest
     bool even = true;
     for (int i = first; i < last; ++i) {
       const uint32_t n = max(decode_list(p, i / p.select_groups, i % p.select_groups).total, 1);
       if (i == first) one = n;
       even = even && n == one;
+      most = max(most, n);
       mine += n * p.kv_per_sel;
     }
     const uint32_t run = wave_prefix_sum(mine);
     const uint32_t head = __builtin_amdgcn_readfirstlane(one);
     even = __all(even && (first == last || one == head));
+    const bool brief = __all(most <= kWholePages);
     if (lane == kWave - 1) {
       s_units[wave] = run;
       s_first[wave] = head;
-      s_even[wave] = even;
+      s_even[wave] = even | brief << 1;
     }
     __syncthreads();
     uint32_t before = 0;
-    bool alike = true;
+    bool alike = true, all_brief = true;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
       if (i < wave) before += s_units[i];
       sh.units += s_units[i];
-      alike = alike && s_even[i] && (s_first[i] == s_first[0] || s_units[i] == 0);
+      all_brief = all_brief && s_even[i] & 2;
+      alike = alike && s_even[i] & 1 && (s_first[i] == s_first[0] || s_units[i] == 0);
     }
     sh.groups = min(gridDim.x, max(1u, sh.units / kMinUnits));
     // Lists of one length are cut into as many shares each, so that no share
     // crosses from one into the next: one that does writes its sums twice.
     const uint32_t all = static_cast<uint32_t>(lists) * p.kv_per_sel;
+    if (all_brief && all <= gridDim.x) {
+      if (w >= all) return;
+      s = w / p.kv_per_sel;
+      const uint32_t pages = max(decode_list(p, s / p.select_groups, s % p.select_groups).total, 1);
+      u = w % p.kv_per_sel * pages;  // of the list's own units
+      end = u + pages;
+    } else {
     if (alike && all <= gridDim.x) sh.groups = all * max(1u, sh.groups / all);
     if (w >= sh.groups) return;
     sh.divide();
@@ -556,6 +549,7 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
     __syncthreads();
     s = __builtin_amdgcn_readfirstlane(s_found[0]);
     base = __builtin_amdgcn_readfirstlane(s_found[1]);
+    }
   }
 
   while (u < end) {
@@ -569,16 +563,15 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
     if constexpr (kCausal) {
       const int64_t per_head = p.tile_info[1];
       h = static_cast<int>(u / per_head);
-      const int4 t = p.tiles[s];
-      b = t.x;
-      pages = t.z;
-      list_first = h * per_head + p.tile_first[s];
-      tg.token0 = p.query_start[b];
-      tg.n_tokens = p.query_start[b + 1] - p.query_start[b];
-      tg.row0 = t.y;
-      const int64_t len = p.seq_len[b];
-      limit0 = static_cast<int>(len) - tg.n_tokens;
-      L = List{nullptr, len, 0, 0, static_cast<int>((len + kPageTokens - 1) / kPageTokens)};
+      const Tile t = p.tiles[s];
+      b = t.batch;
+      pages = t.pages;
+      list_first = h * per_head + t.first;
+      tg.token0 = t.token0;
+      tg.n_tokens = t.n_tokens;
+      tg.row0 = t.row0;
+      limit0 = t.len - t.n_tokens;
+      L = List{nullptr, t.len, 0, 0, (t.len + kPageTokens - 1) / kPageTokens};
     } else {
       for (;;) {
         b = s / p.select_groups;
@@ -627,7 +620,7 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
         wait_fetch();
         Record<D> x;
         read_record<D>(stage, lane, x);
-        wait_reads();
+        wait_lds();
         if (k + 1 < n) fetch(k + 1);
         const int valid = __builtin_amdgcn_readlane(ref.valid, k);
         if (valid > 0)
@@ -643,10 +636,12 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
     const int live_rows = min(kRows, tg.n_tokens * p.group - tg.row0);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const float l = tile_row(st.tail[rt], F::NG, lane);
+      *reinterpret_cast<f32x4*>(&s_tail[wave][r][4 * j]) = st.tail[rt];
+      wait_lds();  // the wave's own
+      const float l = s_tail[wave][r][F::NG];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float add = tile_row(st.tail[rt], (4 * j + i) * F::NC / 32, lane);
+        const float add = s_tail[wave][r][(4 * j + i) * F::NC / 32];
 #pragma unroll
         for (int n = 0; n < F::NC; ++n) st.acc[rt][n][i] += add;
       }
@@ -705,64 +700,70 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
       }
     }
     if (!whole) {
-      const uint32_t w0 = sh.owner(list_first), w1 = sh.owner(list_first + pages - 1);
-      const int shares = static_cast<int>(w1 - w0 + 1);
+      const int w0 = static_cast<int>(sh.owner(list_first));
+      const int w1 = static_cast<int>(sh.owner(list_first + pages - 1));
+      const int shares = w1 - w0 + 1;
       if (last_arrival(p.arrive + w0, shares, &s_last)) {
         const auto record = [&](int i) {
           return p.records + (2 * static_cast<int64_t>(w0 + i) + (i == 0 ? 1 : 0)) * kRecFloats;
         };
-        // Two channels a thread; with threads to spare each takes every
-        // `parts`-th record, and the parts meet in LDS, in order.
-        const int pairs = live_rows * (D / 2);
-        const int parts = min(max(kThreads / pairs, 1), shares);
-        const int part = parts > 1 ? tid / pairs : 0;
+        // A few channels a thread; with threads to spare each takes every
+        // `parts`-th record, and the parts meet in LDS, in order.  One token's
+        // lists are cut into many shares, tiles of rows into few.
+        constexpr int kWide = kCausal ? 4 : 2, kAtOnce = kCausal ? 4 : 8;  // channels, records on their way
+        const int pieces = live_rows * (D / kWide);
+        const int parts = min(max(kThreads / pieces, 1), shares);
+        const int part = parts > 1 ? tid / pieces : 0;
 #pragma unroll 1
-        for (int e = tid - part * pairs; e < pairs; e += kThreads) {
-          const int row = e / (D / 2), ch = e % (D / 2) * 2;
+        for (int e = tid - part * pieces; e < pieces; e += kThreads) {
+          const int row = e / (D / kWide), ch = e % (D / kWide) * kWide;
           // In 64 bits: a share of small weights added to one of a large one
           // loses the same bits every time.
           float top = kNegInf;
-          double sum = 0.0, a = 0.0, b = 0.0;
-          const auto add = [&](float m, float l, float x, float y) {
+          double sum = 0.0, a[kWide] = {};
+          const auto add = [&](float m, float l, const float* x) {
             const float to = fmaxf(top, m);
             const double f = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
             const double g = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
             top = to;
             sum = __builtin_fma(l, f, sum * g);
-            a = __builtin_fma(x, f, a * g);
-            b = __builtin_fma(y, f, b * g);
+#pragma unroll
+            for (int c = 0; c < kWide; ++c) a[c] = __builtin_fma(x[c], f, a[c] * g);
           };
-          constexpr int kAtOnce = 8;  // records on their way
 #pragma unroll 1
           for (int i = part; part < parts && i < shares; i += parts * kAtOnce) {
-            float2 ml[kAtOnce], x[kAtOnce];
+            float2 ml[kAtOnce], x[kAtOnce][kWide / 2];
 #pragma unroll
             for (int n = 0; n < kAtOnce; ++n) {
               const float* z = record(min(i + n * parts, shares - 1));
               ml[n] = load_pair(z + 2 * row);
-              x[n] = load_pair(z + 2 * kRows + row * D + ch);
+#pragma unroll
+              for (int c = 0; c < kWide / 2; ++c) x[n][c] = load_pair(z + 2 * kRows + row * D + ch + 2 * c);
             }
 #pragma unroll
             for (int n = 0; n < kAtOnce; ++n)
-              if (i + n * parts < shares) add(ml[n].x, ml[n].y, x[n].x, x[n].y);
+              if (i + n * parts < shares) add(ml[n].x, ml[n].y, &x[n][0].x);
           }
           if (parts > 1) {  // (one round of the loop)
-            float* to = s_acc + (part * pairs + e) * 4;
+            float* to = s_acc + (part * pieces + e) * (2 + kWide);
             to[0] = top;
             to[1] = static_cast<float>(sum);
-            to[2] = static_cast<float>(a);
-            to[3] = static_cast<float>(b);
+#pragma unroll
+            for (int c = 0; c < kWide; ++c) to[2 + c] = static_cast<float>(a[c]);
             __syncthreads();
             if (part > 0) break;
             for (int n = 1; n < parts; ++n) {
-              const float* z = s_acc + (n * pairs + e) * 4;
-              add(z[0], z[1], z[2], z[3]);
+              const float* z = s_acc + (n * pieces + e) * (2 + kWide);
+              add(z[0], z[1], z + 2);
             }
           }
           const float l = static_cast<float>(sum);
           const int token = (tg.row0 + row) / p.group;
-          store_out2(p, tg.token0 + token, tg.head0 + (tg.row0 + row - token * p.group), D, ch,
-                     sum == 0.0 ? 0.0f : static_cast<float>(a) / l, sum == 0.0 ? 0.0f : static_cast<float>(b) / l);
+#pragma unroll
+          for (int c = 0; c < kWide; c += 2)
+            store_out2(p, tg.token0 + token, tg.head0 + (tg.row0 + row - token * p.group), D, ch + c,
+                       sum == 0.0 ? 0.0f : static_cast<float>(a[c]) / l,
+                       sum == 0.0 ? 0.0f : static_cast<float>(a[c + 1]) / l);
         }
       }
     }
@@ -776,8 +777,7 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
 }
 
 // ---- the tiles of a ragged batch of query tokens ------------------------------------
-// Tile: `rows` rows (token * group + head) of one sequence, for every KV head.
-// Its pages end with the last one that its last row sees.  One workgroup.
+// A tile's pages end with the last one that its last row sees.  One workgroup.
 constexpr int kTileThreads = 1024;
 
 __global__ __launch_bounds__(kTileThreads) void tiles_kernel(const Params p, int rows) {
@@ -829,6 +829,7 @@ __global__ __launch_bounds__(kTileThreads) void tiles_kernel(const Params p, int
     if (tid == 0) flag_status(p.status, kStatusBadLength);
   }
   int64_t units = 0;
+  int longest = 0;
   for (int64_t x0 = 0; x0 < tiles; x0 += kTileThreads) {
     const int64_t x = x0 + tid;
     int b = 0, row0 = 0, pages = 0;
@@ -854,14 +855,22 @@ __global__ __launch_bounds__(kTileThreads) void tiles_kernel(const Params p, int
     int64_t sum;
     const int64_t pre = scan(pages, sum);
     if (x < tiles) {
-      p.tiles[x] = make_int4(b, row0, pages, 0);
-      p.tile_first[x] = units + pre;
+      const int token0 = p.query_start[b];
+      p.tiles[x] = Tile{units + pre, b, row0, pages, p.query_start[b + 1] - token0, token0, p.seq_len[b]};
     }
     units += sum;
+    longest = max(longest, pages);
   }
+  for (int d = 1; d < kWave; d *= 2) longest = max(longest, __shfl_xor(longest, d));
+  __syncthreads();
+  if (lane == 0) s_wave[wave] = longest;
+  __syncthreads();
+  int64_t most = 0;
+  for (int i = 0; i < kTileThreads / kWave; ++i) most = max(most, s_wave[i]);
   if (tid == 0) {
     p.tile_info[0] = tiles;
     p.tile_info[1] = units;
+    p.tile_info[2] = most;
   }
 }
 
@@ -895,7 +904,7 @@ Form form_of(bool prompt, int64_t tokens, int64_t batch, int group, int head_dim
 }
 
 struct Layout {
-  size_t records, info, first, tiles, bytes;
+  size_t records, info, tiles, bytes;
 };
 
 Layout layout(const Plan& pl, int64_t batch, int64_t tokens, int group) {
@@ -903,9 +912,8 @@ Layout layout(const Plan& pl, int64_t batch, int64_t tokens, int group) {
   const int64_t tiles = max_tiles(batch, tokens, group, pl.rows);
   l.records = kMaxGroups * sizeof(int32_t);  // behind the arrival counters
   l.info = (l.records + pl.records + 255) / 256 * 256;
-  l.first = l.info + 256;
-  l.tiles = (l.first + tiles * sizeof(int64_t) + 255) / 256 * 256;
-  l.bytes = l.tiles + tiles * sizeof(int4);
+  l.tiles = l.info + 256;
+  l.bytes = l.tiles + tiles * sizeof(Tile);
   return l;
 }
 
@@ -981,8 +989,7 @@ hipError_t launch_kv4_attention(const Kv4AttnLaunch& a, hipStream_t stream) {
   p.arrive = reinterpret_cast<int32_t*>(ws);
   p.records = reinterpret_cast<float*>(ws + l.records);
   p.tile_info = reinterpret_cast<int64_t*>(ws + l.info);
-  p.tile_first = reinterpret_cast<int64_t*>(ws + l.first);
-  p.tiles = reinterpret_cast<int4*>(ws + l.tiles);
+  p.tiles = reinterpret_cast<Tile*>(ws + l.tiles);
   if (a.query_start) {
     const hipError_t e = launch_tiles(p, pl.rows, stream);
     if (e != hipSuccess) return e;

@@ -22,6 +22,8 @@ constexpr float kLowest = -3.0e38f;  // of masked scores: finite, so that a fact
 constexpr float kLog2e = 1.4426950408889634f;
 
 
+struct Tile;
+
 struct Params {
   const uint8_t* pool;
   const int32_t* table;
@@ -35,9 +37,8 @@ struct Params {
   int32_t* status;
   int32_t* arrive;
   float* records;
-  int64_t* tile_info;  // prompt: [0] tiles, [1] units of one KV head
-  int64_t* tile_first; // units before a tile
-  int4* tiles;         // (sequence, first row, pages, -)
+  int64_t* tile_info;  // prompt: [0] tiles, [1] units of one KV head, [2] pages of the longest
+  Tile* tiles;
   int64_t num_pages;
   int64_t q_stride;
   int32_t tokens;
@@ -167,23 +168,15 @@ __device__ inline float ldexp2(float x, int e) { return __builtin_ldexpf(x, e); 
 // The pages of all lists form one row of units; workgroup w of `groups` takes
 // units [begin(w), begin(w + 1)), whatever lists they belong to.
 
-struct Share {
-  int64_t units;   // of the whole launch
-  int64_t groups;  // workgroups that take part
-  __device__ inline int64_t begin(int64_t w) const { return units * w / groups; }
-  __device__ inline int64_t owner(int64_t u) const { return ((u + 1) * groups - 1) / units; }
-};
-
-// The same in 32 bits, for fewer than 2^31 units and at most 4096 groups: a
-// 64-bit division takes longer than a small list.
-struct SmallShare {
-  uint32_t units;
-  uint32_t groups;
+struct SmallShare {  // fewer than 2^31 units, at most 4096 groups
+  uint32_t units;    // of the whole launch
+  uint32_t groups;   // workgroups that take part
   uint32_t each, rest;  // units = each * groups + rest
   __device__ inline void divide() {
     each = units / groups;
     rest = units - each * groups;
   }
+  // floor(units * w / groups)
   __device__ inline uint32_t begin(uint32_t w) const { return each * w + rest * w / groups; }
   __device__ inline uint32_t owner(uint32_t u) const {
     uint32_t w = static_cast<uint32_t>(static_cast<float>(u) * (static_cast<float>(groups) / static_cast<float>(units)));
@@ -194,6 +187,65 @@ struct SmallShare {
   }
 };
 
+struct Share {
+  int64_t units;
+  int64_t groups;
+  __device__ inline int64_t begin(int64_t w) const { return units * w / groups; }
+  __device__ inline int64_t owner(int64_t u) const { return ((u + 1) * groups - 1) / units; }
+};
+
+// Lists of at most this many pages, a workgroup for each, are not cut: the
+// shares' sums would take longer to meet than the pages to be attended.
+constexpr int kWholePages = 16;
+
+// `rows` rows (token * group + head) of one sequence, for every KV head.
+struct Tile {
+  int64_t first;   // unit of its first page, for the first head
+  int batch;       // sequence
+  int row0;        // its first row of the sequence
+  int pages;       // that its last row sees
+  int n_tokens;    // query tokens of the sequence
+  int token0;      // the first of them
+  int len;         // tokens of the sequence
+};
+static_assert(sizeof(Tile) == 32, "two 16-byte loads");
+
+// The tile of the unit, 0 <= at < tile_info[1]: each lane compares one of 64
+// candidates.
+__device__ inline int find_tile(const Params& p, int64_t at, int lane) {
+  int lo = 0, n = static_cast<int>(p.tile_info[0]);
+  while (n > 1) {
+    const int step = (n + kWave - 1) / kWave;
+    const bool below = lane * step < n && p.tiles[lo + lane * step].first <= at;
+    const int k = __popcll(__ballot(below)) - 1;
+    lo += k * step;
+    n = min(step, n - k * step);
+  }
+  return lo;
+}
+
+// The first list and unit of workgroup w and the end of its share.
+struct Start {
+  int s;   // tile
+  int64_t u, end;
+  bool any;
+};
+__device__ inline Start start_share(const Params& p, Share& sh, int64_t w, int min_units, int lane) {
+  const int64_t tiles = p.tile_info[0], per_head = p.tile_info[1], longest = p.tile_info[2];
+  sh.units = per_head * p.kv_heads;
+  if (sh.units <= 0) return Start{0, 0, 0, false};
+  if (tiles * p.kv_heads <= static_cast<int64_t>(gridDim.x) && longest <= kWholePages) {
+    if (w >= tiles * p.kv_heads) return Start{0, 0, 0, false};
+    const int s = static_cast<int>(w) % static_cast<int>(tiles);
+    const int64_t u = static_cast<int>(w) / static_cast<int>(tiles) * per_head + p.tiles[s].first;
+    return Start{s, u, u + p.tiles[s].pages, true};
+  }
+  sh.groups = min<int64_t>(gridDim.x, max<int64_t>(1, sh.units / min_units));
+  if (w >= sh.groups) return Start{0, 0, 0, false};
+  const int64_t u = sh.begin(w);
+  return Start{find_tile(p, u % per_head, lane), u, sh.begin(w + 1), true};
+}
+
 struct Target {
   int64_t token0;  // first query row of the sequence
   int n_tokens;
@@ -202,7 +254,7 @@ struct Target {
 };
 
 // The tiles of `rows` rows each of a batch of query tokens (kv4_attention.hip)
-// into p.tiles, p.tile_first and p.tile_info.
+// into p.tiles and p.tile_info.
 hipError_t launch_tiles(const Params& p, int rows, hipStream_t stream);
 int64_t max_tiles(int64_t batch, int64_t tokens, int group, int rows);
 

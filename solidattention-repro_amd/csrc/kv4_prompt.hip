@@ -352,31 +352,19 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
   const int64_t w = blockIdx.x;
   const int64_t per_head = p.tile_info[1];
   const int tiles = static_cast<int>(p.tile_info[0]);
-  Share sh{per_head * p.kv_heads, 0};
-  if (sh.units <= 0) return;
-  sh.groups = min<int64_t>(gridDim.x, max<int64_t>(1, sh.units / kMinUnits));
-  if (w >= sh.groups) return;
-  int64_t u = sh.begin(w);
-  const int64_t end = sh.begin(w + 1);
-  int s = 0;
-  {
-    const int64_t at = u % per_head;
-    int hi = tiles;
-    while (hi - s > 1) {
-      const int mid = (s + hi) / 2;
-      if (p.tile_first[mid] <= at) s = mid;
-      else hi = mid;
-    }
-  }
+  Share sh{};
+  const Start start = start_share(p, sh, w, kMinUnits, lane);
+  if (!start.any) return;
+  int s = start.s;
+  int64_t u = start.u;
+  const int64_t end = start.end;
 
   while (u < end) {
     const int head = static_cast<int>(u / per_head);
-    const int4 tile = p.tiles[s];
-    const int b = tile.x, row0 = tile.y, pages = tile.z;
-    const int64_t list_first = head * per_head + p.tile_first[s];
-    const int token0 = p.query_start[b];
-    const int n_tokens = p.query_start[b + 1] - token0;
-    const int len = p.seq_len[b];
+    const Tile tile = p.tiles[s];
+    const int b = tile.batch, row0 = tile.row0, pages = tile.pages;
+    const int64_t list_first = head * per_head + tile.first;
+    const int token0 = tile.token0, n_tokens = tile.n_tokens, len = tile.len;
     const List L{nullptr, len, 0, 0, (len + kPageTokens - 1) / kPageTokens};
     const int p0 = static_cast<int>(u - list_first);
     const int p1 = static_cast<int>(min<int64_t>(pages, p0 + (end - u)));
@@ -385,6 +373,27 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
     const int row = row0 + wave * kWaveRows + lane % 32;
     const bool live = lane % 32 < mine;
     const int token = row / p.group, qh = head * p.group + row % p.group;
+
+    const int64_t page_bytes = static_cast<int64_t>(p.kv_heads) * F::kRecord;
+    const uint8_t* pool = p.pool + static_cast<int64_t>(head) * F::kRecord;
+    PageRef ref{0, 0};
+    int looked = p0 - 2 * kWave;  // the lanes hold pages [looked, looked + 64)
+    Raw<D> raw[2];
+    int raw_valid[2];
+    const auto get = [&](int i) {  // pages i and i + 1 into registers (the second may not be there)
+      if (i + 1 - looked >= kWave) {
+        looked = i;
+        ref = PageRef{0, 0};
+        if (i + lane < p1) ref = resolve(p, b, L, i + lane);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int64_t page = __builtin_amdgcn_readlane(ref.page, i + s - looked);
+        fetch<D>(pool + page * page_bytes, place, wave, raw[s]);
+        raw_valid[s] = __builtin_amdgcn_readlane(ref.valid, i + s - looked);
+      }
+    };
+    get(p0);  // on their way while the rows are read
 
     State<D> st;
     st.m = kNegInf;
@@ -424,25 +433,6 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
       for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(st.q[i]));  // made once, not anew for every page
     }
 
-    const int64_t page_bytes = static_cast<int64_t>(p.kv_heads) * F::kRecord;
-    const uint8_t* pool = p.pool + static_cast<int64_t>(head) * F::kRecord;
-    PageRef ref{0, 0};
-    int looked = p0 - 2 * kWave;  // the lanes hold pages [looked, looked + 64)
-    Raw<D> raw[2];
-    int raw_valid[2];
-    const auto get = [&](int i) {  // pages i and i + 1 into registers (the second may not be there)
-      if (i + 1 - looked >= kWave) {
-        looked = i;
-        ref = PageRef{0, 0};
-        if (i + lane < p1) ref = resolve(p, b, L, i + lane);
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int64_t page = __builtin_amdgcn_readlane(ref.page, i + s - looked);
-        fetch<D>(pool + page * page_bytes, place, wave, raw[s]);
-        raw_valid[s] = __builtin_amdgcn_readlane(ref.valid, i + s - looked);
-      }
-    };
     const auto put = [&](int i, Page<D>* page) {  // pages i and i + 1, which are in registers; then the next two into them
 #pragma unroll
       for (int s = 0; s < 2; ++s) convert<D>(raw[s], page[s], raw_valid[s], place, wave, lane);
@@ -452,7 +442,6 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
     // in pairs; sets grow from one pair, so that the first is not waited for
     // longer.  (One place in the code for each: two would copy the sums
     // between them.)
-    get(p0);
     put(p0, s_page[0]);
     lds_barrier();
     const int late = wave / (kWaves / 2) * 2;
