@@ -110,7 +110,7 @@ __device__ inline void read_record(const uint8_t* slot, int lane, Record<D>& x) 
 }
 
 // The value operand of channel n of every row: slots 8j.. of tiles 0 and 1.
-template <int D, int N>
+template <int D, int N, int kCentre>
 __device__ inline half8 value_operand(const Record<D>& x) {
   uint32_t w[4];
 #pragma unroll
@@ -126,8 +126,8 @@ __device__ inline half8 value_operand(const Record<D>& x) {
       p01 = __builtin_amdgcn_perm(x.vc[T][kStep + kWord], x.vc[T][kWord], kSel);
       p23 = __builtin_amdgcn_perm(x.vc[T][3 * kStep + kWord], x.vc[T][2 * kStep + kWord], kSel);
     }
-    w[2 * T] = scaled_codes<N % 4>(p01, x.vs[2 * T]);
-    w[2 * T + 1] = scaled_codes<N % 4>(p23, x.vs[2 * T + 1]);
+    w[2 * T] = scaled_codes<N % 4, kCentre>(p01, x.vs[2 * T]);
+    w[2 * T + 1] = scaled_codes<N % 4, kCentre>(p23, x.vs[2 * T + 1]);
   }
   return as_half8(w[0], w[1], w[2], w[3]);
 }
@@ -260,16 +260,16 @@ __device__ inline uint32_t slot_mask(int q, int j, int valid) {
   return (t < valid ? 0x0000FFFFu : 0u) | (t + 1 < valid ? 0xFFFF0000u : 0u);
 }
 
-template <int D, int RT, int N>
-__device__ inline void add_values(const Record<D>& x, const half8 (&ph)[RT], const half8 (&pl)[RT], bool fine,
+template <int D, int RT, bool kFine, int N>
+__device__ inline void add_values(const Record<D>& x, const half8 (&ph)[RT], const half8 (&pl)[RT],
                                   State<D, RT>& st) {
-  const half8 v = value_operand<D, N>(x);
+  const half8 v = value_operand<D, N, kFine ? 8 : 0>(x);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     st.acc[rt][N] = mfma(v, ph[rt], st.acc[rt][N]);
-    if (fine) st.acc[rt][N] = mfma(v, pl[rt], st.acc[rt][N]);
+    if constexpr (kFine) st.acc[rt][N] = mfma(v, pl[rt], st.acc[rt][N]);
   }
-  if constexpr (N + 1 < Format<D>::NC) add_values<D, RT, N + 1>(x, ph, pl, fine, st);
+  if constexpr (N + 1 < Format<D>::NC) add_values<D, RT, kFine, N + 1>(x, ph, pl, st);
 }
 
 // Attends one page: `valid` tokens, the first at position pos; kCausal: a
@@ -375,8 +375,24 @@ __device__ inline void attend(Record<D>& x, int valid, int pos, int first_limit,
       x.vs[i] &= mask;
       x.vm[i] &= mask;
     }
-    w[i] = r < F::NG ? x.vm[i] : r == F::NG ? 0x3C003C00u : 0u;
+    w[i] = x.vm[i];
   }
+  // For fp32 the codes enter less 8, and the minima with 8 scales, in two
+  // parts: sums of one sign, whose rounding errors add up, would cancel in the
+  // output (64 blocks of 32: 6e-6 of it, against 6e-7; 46 -> 48 us).
+  uint32_t low[4];
+  if constexpr (kFine) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const half2_t scales = as_half2(__shfl(x.vs[i], 16 * j + r % F::NG * (32 / F::NC)));
+      half2_t sum, rest;
+      add_eight_times(as_half2(w[i]), scales, sum, rest);
+      w[i] = bits_of(sum);
+      low[i] = r < F::NG ? bits_of(rest) : 0u;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = r < F::NG ? w[i] : r == F::NG ? 0x3C003C00u : 0u;
   // A NaN minimum in a page that only some rows see wholly: 0 * NaN would
   // reach the others, so it is taken out and added to the rows that see it.
   if constexpr (kCausal) {
@@ -385,7 +401,10 @@ __device__ inline void attend(Record<D>& x, int valid, int pos, int first_limit,
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
         const bool nan = ((w[n / 2] >> (16 * (n % 2))) & 0x7fffu) > 0x7c00u;
-        if (nan) w[n / 2] &= n % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+        if (nan) {
+          w[n / 2] &= n % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+          if constexpr (kFine) low[n / 2] &= n % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+        }
         any |= nan;
       }
       if (__any(any)) {
@@ -414,9 +433,12 @@ __device__ inline void attend(Record<D>& x, int valid, int pos, int first_limit,
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     st.tail[rt] = mfma(last, ph[rt], st.tail[rt]);
-    if constexpr (kFine) st.tail[rt] = mfma(last, pl[rt], st.tail[rt]);
+    if constexpr (kFine) {
+      st.tail[rt] = mfma(last, pl[rt], st.tail[rt]);
+      st.tail[rt] = mfma(as_half8(low[0], low[1], low[2], low[3]), ph[rt], st.tail[rt]);
+    }
   }
-  add_values<D, RT, 0>(x, ph, pl, kFine, st);
+  add_values<D, RT, kFine, 0>(x, ph, pl, st);
 }
 
 // ---- shares of the row of units ---------------------------------------------------

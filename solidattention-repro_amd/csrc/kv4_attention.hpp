@@ -139,10 +139,17 @@ __device__ inline uint32_t and_or(uint32_t x, uint32_t mask, uint32_t base) {
   return d;
 }
 
-// Nibbles 0 and 1 of both halves as FP16 integers: moved into the mantissa of
-// 1024.0 (bits 0..3) or 64.0 (bits 4..7), which is then taken off (exact).
-__device__ inline half2_t low_nibbles(uint32_t w) { return as_half2(and_or(w, 0x000F000Fu, 0x64006400u)) - half2_t{1024, 1024}; }
-__device__ inline half2_t high_nibbles(uint32_t w) { return as_half2(and_or(w, 0x00F000F0u, 0x54005400u)) - half2_t{64, 64}; }
+// Nibbles 0 and 1 of both halves as FP16 integers (less kCentre): moved into
+// the mantissa of 1024.0 (bits 0..3) or 64.0 (bits 4..7), which is then taken
+// off (exact).
+template <int kCentre = 0>
+__device__ inline half2_t low_nibbles(uint32_t w) {
+  return as_half2(and_or(w, 0x000F000Fu, 0x64006400u)) - half2_t{1024 + kCentre, 1024 + kCentre};
+}
+template <int kCentre = 0>
+__device__ inline half2_t high_nibbles(uint32_t w) {
+  return as_half2(and_or(w, 0x00F000F0u, 0x54005400u)) - half2_t{64 + kCentre, 64 + kCentre};
+}
 
 // 8 nibbles in the order (0,4), (1,5), (2,6), (3,7).
 __device__ inline half8 key_codes(uint32_t w) {
@@ -150,12 +157,20 @@ __device__ inline half8 key_codes(uint32_t w) {
                   bits_of(high_nibbles(w >> 8)));
 }
 
-// Nibble n (0..3) of both halves as FP16 integers times the pair of scales
-// (exact: 4 + 7 bits).
-template <int N>
+// Nibble n (0..3) of both halves as FP16 integers, less kCentre, times the
+// pair of scales (exact: 4 + 7 bits).
+template <int N, int kCentre>
 __device__ inline uint32_t scaled_codes(uint32_t y, uint32_t scales) {
   const uint32_t w = N < 2 ? y : y >> 8;
-  return bits_of((N % 2 == 0 ? low_nibbles(w) : high_nibbles(w)) * as_half2(scales));
+  return bits_of((N % 2 == 0 ? low_nibbles<kCentre>(w) : high_nibbles<kCentre>(w)) * as_half2(scales));
+}
+
+// a + 8 b = sum + rest, without an error
+__device__ inline void add_eight_times(half2_t a, half2_t b, half2_t& sum, half2_t& rest) {
+  const half2_t c = b * half2_t{8, 8};
+  sum = a + c;
+  const half2_t d = sum - a;
+  rest = (a - (sum - d)) + (c - d);
 }
 
 __device__ inline f32x4 mfma(half8 a, half8 b, f32x4 c) {

@@ -6,7 +6,10 @@
 // its 8 waves, and all of them attend the same page.  The page's 8 KB of codes
 // are turned into FP16 once, scale * code + minimum rounded once (2^-11
 // relative, as an FP16 cache's own values), by all waves together, into LDS in
-// the order of the operands of v_mfma_f32_32x32x16_f16:
+// the order of the operands of v_mfma_f32_32x32x16_f16.  For FP16 queries,
+// whose output keeps more bits than BF16's, the keys enter as scale * code
+// (exact) and their minima by a product more with the sums of q (the output's
+// error falls from 3.3e-4 to 3.0e-4 of it, the time rises by 5%).
 //   scores   rows = tokens, columns = query rows: lane (column c = lane % 32,
 //            half h = lane / 32) holds tokens 8 (i / 4) + 4 h + i % 4, i < 16.
 //   values   rows = channels, columns = query rows; product step s runs over
@@ -51,6 +54,7 @@ struct Page {
   using F = Format<D>;
   half8 k[D / 16][kWave];     // product step, lane of the operand
   half8 v[D / 32][2][kWave];  // channels' tile, product step, lane
+  half8 mins[kPageTokens];    // the keys' minima, the NG groups' over and over
   uint32_t nan[2][F::NG];     // bit t: token 16 T + t of the values' group is NaN
   uint32_t valid;             // tokens (0: no page); right behind the words of `nan`
 };
@@ -130,21 +134,36 @@ __device__ inline uint32_t scaled(half2_t c, half2_t s, half2_t m) { return bits
 // Turns the thread's part into operands.  A NaN minimum of the values goes
 // into page.nan instead (0 * NaN would reach the rows that do not see the
 // token) and its group enters as 0.
-template <int D>
+template <int D, bool kExact>
 __device__ inline void convert(const Raw<D>& x, Page<D>& page, int valid, const Place<D>& at, int wave, int lane) {
   using F = Format<D>;
   const int r = lane % 16, j = lane / 16, T = wave % 2, half = wave / 2 % 2;
   uint8_t* to = reinterpret_cast<uint8_t*>(&page) + at.to;
   if (wave < 4) {
     if (wave == 0 && lane == 0) page.valid = valid;
+    if (kExact && j == 0) {
+      if constexpr (D == 64) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          reinterpret_cast<uint16_t*>(&page.mins[16 * T + r])[2 * i + half] = static_cast<uint16_t>(x.m[0]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) reinterpret_cast<uint32_t*>(&page.mins[16 * T + r])[2 * i + half] = x.m[0];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < F::NG / 2; ++i) {  // the row's next word is the other half of a product step
       const uint32_t w = x.codes[i];
       const half2_t s = as_half2(x.s[i] * 0x10001u);
-      const half2_t m = as_half2((i % 2 ? x.m[0] >> 16 : x.m[0] & 0xFFFFu) * 0x10001u);
-      *reinterpret_cast<half8*>(to + i * 32 * 16) =
-          as_half8(scaled(low_nibbles(w), s, m), scaled(high_nibbles(w), s, m), scaled(low_nibbles(w >> 8), s, m),
-                   scaled(high_nibbles(w >> 8), s, m));
+      half8& k = *reinterpret_cast<half8*>(to + i * 32 * 16);
+      if constexpr (kExact) {
+        k = as_half8(bits_of(low_nibbles(w) * s), bits_of(high_nibbles(w) * s), bits_of(low_nibbles(w >> 8) * s),
+                     bits_of(high_nibbles(w >> 8) * s));
+      } else {
+        const half2_t m = as_half2((i % 2 ? x.m[0] >> 16 : x.m[0] & 0xFFFFu) * 0x10001u);
+        k = as_half8(scaled(low_nibbles(w), s, m), scaled(high_nibbles(w), s, m), scaled(low_nibbles(w >> 8), s, m),
+                     scaled(high_nibbles(w >> 8), s, m));
+      }
     }
     return;
   }
@@ -195,6 +214,7 @@ __device__ inline void convert(const Raw<D>& x, Page<D>& page, int valid, const 
 template <int D>
 struct State {
   half8 q[D / 16];
+  half8 sums;        // of the row's groups, in two parts: the minima's operand
   f32x16 acc[D / 32];
   float m, l, factor;
   int limit;        // last position the lane's row sees
@@ -203,7 +223,7 @@ struct State {
 };
 
 // Attends two pages, the first one's tokens from position pos on.
-template <int D>
+template <int D, bool kExact>
 __device__ inline void attend(const Page<D> (&page)[2], int pos, int lane, State<D>& st) {
   constexpr int kNG = Format<D>::NG, kNC = Format<D>::NC, kOps = D / 16;
   const int h = lane / 32;
@@ -213,18 +233,22 @@ __device__ inline void attend(const Page<D> (&page)[2], int pos, int lane, State
   // The operands are read ahead of the products that take them, the values'
   // before the exponentials: read one by one, the LDS's latency took half of
   // the time.
-  half8 op[kOps];
+  half8 op[kOps], mins{};
   f32x16 z[2];
 #pragma unroll
   for (int i = 0; i < kOps; ++i) op[i] = page[0].k[i][lane];
+  if constexpr (kExact) mins = page[0].mins[lane % 32];
   __builtin_amdgcn_sched_barrier(0);
   z[0] = f32x16{};
+  if constexpr (kExact) z[0] = mfma32(mins, st.sums, z[0]);
 #pragma unroll
   for (int i = 0; i < kOps; ++i) z[0] = mfma32(op[i], st.q[i], z[0]);
 #pragma unroll
   for (int i = 0; i < kOps; ++i) op[i] = page[1].k[i][lane];
+  if constexpr (kExact) mins = page[1].mins[lane % 32];
   __builtin_amdgcn_sched_barrier(0);
   z[1] = f32x16{};
+  if constexpr (kExact) z[1] = mfma32(mins, st.sums, z[1]);
 #pragma unroll
   for (int i = 0; i < kOps; ++i) z[1] = mfma32(op[i], st.q[i], z[1]);
 #pragma unroll
@@ -340,7 +364,7 @@ __device__ inline void store_row(const Params& p, int64_t token, int head, const
   }
 }
 
-template <int D>
+template <int D, bool kExact>
 __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p) {
   using F = Format<D>;
   __shared__ Page<D> s_page[2][kBatch];
@@ -429,13 +453,29 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
           const float v = x[i][n / 2 + (n % 2) * 4];  // operand order (0,4), (1,5), ...
           st.q[i][n] = static_cast<_Float16>(ldexp2(p.qscale < 0.0f ? -v : v, -e));
         }
+      if constexpr (kExact) {
+        float sum[F::NG / 2] = {};  // of groups h, h + 2, .. (word 2 i + h is of group (2 i + h) % NG)
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int n = 0; n < 8; ++n) sum[i % (F::NG / 2)] += static_cast<float>(st.q[i][n]);
+        st.sums = half8{};
+#pragma unroll
+        for (int g = 0; g < F::NG; ++g) {
+          const float other = __shfl_xor(sum[g / 2], 32);
+          const float v = h != 0 ? 0.0f : g % 2 == 0 ? sum[g / 2] : other;
+          st.sums[g] = static_cast<_Float16>(v);
+          st.sums[F::NG + g] = static_cast<_Float16>(v - static_cast<float>(st.sums[g]));
+        }
+        asm volatile("" : "+v"(st.sums));
+      }
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(st.q[i]));  // made once, not anew for every page
     }
 
     const auto put = [&](int i, Page<D>* page) {  // pages i and i + 1, which are in registers; then the next two into them
 #pragma unroll
-      for (int s = 0; s < 2; ++s) convert<D>(raw[s], page[s], raw_valid[s], place, wave, lane);
+      for (int s = 0; s < 2; ++s) convert<D, kExact>(raw[s], page[s], raw_valid[s], place, wave, lane);
       if (i + 2 < p1) get(i + 2);
     };
     // Pages [a, z) are attended out of one set while [z, y) go into the other,
@@ -450,7 +490,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
       for (int i = 0; i < max(z - a, y - z) + late; i += 2) {
         if (i >= late && z + i - late < y) put(z + i - late, s_page[set ^ 1] + (i - late));
         if (a + i < z && (a + i) * kPageTokens <= st.last)
-          attend<D>(*reinterpret_cast<const Page<D>(*)[2]>(s_page[set] + i), (a + i) * kPageTokens, lane, st);
+          attend<D, kExact>(*reinterpret_cast<const Page<D>(*)[2]>(s_page[set] + i), (a + i) * kPageTokens, lane, st);
       }
       lds_barrier();
       a = z;
@@ -508,8 +548,9 @@ size_t prompt_record_floats(int head_dim) { return static_cast<size_t>(kWaves) *
 
 hipError_t launch_prompt_tiles(const Params& p, int head_dim, hipStream_t stream) {
   const dim3 grid(prompt_groups());
-  if (head_dim == 64) hipLaunchKernelGGL(kv4_prompt_kernel<64>, grid, dim3(kThreads), 0, stream, p);
-  if (head_dim == 128) hipLaunchKernelGGL(kv4_prompt_kernel<128>, grid, dim3(kThreads), 0, stream, p);
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, p); };
+  if (head_dim == 64) launch(p.type == kF16 ? kv4_prompt_kernel<64, true> : kv4_prompt_kernel<64, false>);
+  if (head_dim == 128) launch(p.type == kF16 ? kv4_prompt_kernel<128, true> : kv4_prompt_kernel<128, false>);
   return hipGetLastError();
 }
 
