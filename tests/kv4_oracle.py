@@ -93,22 +93,28 @@ def attend(q, k, v, scale):
         return p @ v / p.sum(-1, keepdims=True), float(np.abs(v).max())
 
 
-def error_bound(q, k, v, scale, dtype, eps):
+def error_bound(q, k, v, scale, dtype, eps, rounded=False):
     """How far a row's output may be off, absolute, for q [rows][d] on k, v [tokens][d] (eps: half a step of the
     output's type, relative).
 
-    Scores: a group's 32 products are summed in fp32 together with -64 sum q, an error of at most 33 * 2^-24 of the
-    sum of the magnitudes, |q| (64 + 15) scale of the group; the groups' sums add 8 more roundings; fp32 queries in two FP16 parts
-    are off by 2^-22 of the row's largest.  With |k| <= kmax and scales <= 2 kmax / 15 that is at most
-    2^-17 * scale * sum|q| * 12 kmax in the exponent, and a relative change of each probability by as much.
+    Scores: a group's 32 products of q and codes are exact and summed in 32 bits (33 roundings), multiplied by the
+    scale and added to the other groups' and the minima's (at most 16 more); with |k| <= kmax a scaled code is at most
+    2 kmax and a minimum kmax, so that is at most 49 * 2^-24 * 3 kmax sum|q|.  Queries and their groups' sums enter in
+    two FP16 parts: 2^-22 of the row's largest for each channel, for rows whose mean magnitude is at least 1/128 of
+    their largest at most 2^-15 * 3 kmax sum|q|.  Both together are below 2^-17 * 12 kmax sum|q|, times the scale in the
+    exponent, and as much in a probability, relative.
     Probabilities rounded to FP16 (16-bit types) are off by 2^-11, in two FP16 parts by 2^-22; numerator and denominator
-    both.  Sums of up to 2^17 terms in fp32 on the matrix cores, in chunks: 2^-18."""
+    both.  Sums of up to 2^17 terms in 32 bits on the matrix cores, in chunks: 2^-18.
+
+    rounded: several tokens a sequence in 16-bit types, whose keys and values may be rounded to FP16: 2^-11 of every
+    key's element in the exponent, and 2^-11 of the values."""
     if k.shape[0] == 0:
         return np.zeros((q.shape[0], 1))
     kmax, vmax = np.abs(k).max(), np.abs(v).max()
-    delta = 2.0 ** -17 * scale * np.abs(q).sum(-1, keepdims=True) * 12 * kmax
+    rounded = rounded and dtype != "fp32"
+    delta = (2.0 ** -17 * 12 + (2.0 ** -11 if rounded else 0)) * scale * np.abs(q).sum(-1, keepdims=True) * kmax
     prob = 2.0 ** -22 if dtype == "fp32" else 2.0 ** -11
-    out = (2 * np.expm1(delta) + 2 * prob + 2.0 ** -18) * vmax
+    out = (2 * np.expm1(delta) + 2 * prob + 2.0 ** -18 + (2.0 ** -11 if rounded else 0)) * vmax
     return out + eps * vmax
 
 

@@ -99,6 +99,36 @@ def test_decode_batches(hip, B):
     check_decode(c, q, out, "fp32", 128 ** -0.5)
 
 
+@pytest.mark.parametrize("d,lengths", [(64, [1, 512, 0, 40]), (128, [300] * 5), (128, [512, 511]), (256, [33, 64, 2]),
+                                       (128, [513, 20]), (64, [2000] * 3), (128, [700] * 40)])
+def test_decode_short_and_equal_lists(hip, d, lengths):
+    """Lists of up to 16 pages with a workgroup each, one page more, and lists of one length, whose shares end with
+    them; whole sequences and selected blocks."""
+    c = Cache(hip, lengths, 4, d, 2, seed=7)
+    q = query(8, len(lengths), 8, d, "fp32")
+    status = ints([0])
+    ws = hip.kv4_attention_workspace(c.kv)
+    out = hip.kv4_decode_attention(c.kv, q.cuda(), 0.1, workspace=ws, status=status)
+    check_decode(c, q, out, "fp32", 0.1)
+    counts = np.stack([np.minimum(3, np.array(lengths) // 32)] * 2, 1)
+    selected = np.tile(np.arange(3), (len(lengths), 2, 1))
+    out = hip.kv4_decode_attention(c.kv, q.cuda(), 0.1, ints(selected), ints(counts), workspace=ws, status=status)
+    check_decode(c, q, out, "fp32", 0.1, selected, counts, 2)
+    assert int(status) == 0
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prompt_short_lists(hip, d, dtype):
+    """Tiles of up to 16 pages with a workgroup each, in tiles of few rows and of many, and tiles of one page more."""
+    for lengths, new in (([512, 40, 3], [4, 2, 3]), ([512, 100], [512, 100]), ([513, 100], [3, 4]), ([530], [400])):
+        c = Cache(hip, lengths, 2, d, 4, seed=6)
+        start = np.concatenate([[0], np.cumsum(new)])
+        q = query(9, int(start[-1]), 8, d, dtype)
+        out = hip.kv4_prompt_attention(c.kv, q.cuda(), ints(start), d ** -0.5)
+        check_prompt(c, q, start, out, dtype, d ** -0.5)
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("d,heads,group,groups", [(64, 4, 2, 4), (128, 8, 2, 8), (128, 8, 4, 1), (128, 4, 1, 2),
                                                   (256, 2, 8, 2)])
@@ -133,8 +163,8 @@ def check_prompt(c, q, start, out, dtype, scale, untouched=None):
                 seen = n - m + i + 1
                 qq, got = qn[start[b] + i, rows], on[start[b] + i, rows]
                 want, _ = K.attend(qq, k[:max(seen, 0)], v[:max(seen, 0)], scale)
-                check(got, want, K.error_bound(qq, k[:max(seen, 0)], v[:max(seen, 0)], scale, dtype, EPS[dtype]) + 1e-30,
-                      (b, h, i))
+                bound = K.error_bound(qq, k[:max(seen, 0)], v[:max(seen, 0)], scale, dtype, EPS[dtype], rounded=True)
+                check(got, want, bound + 1e-30, (b, h, i))
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
