@@ -780,7 +780,9 @@ size_t sa_hip_kv4_attention_workspace_bytes(const sa_paged_kv* kv, int32_t query
  * every token of the sequence.  query ([batch][query_heads][head_dim], q_stride elements
  * between tokens) and out (contiguous) of `type`; query 16-byte aligned in
  * every row.  fp32 softmax and sums; fp32 queries enter the matrix cores as
- * two FP16 parts.  A sequence without tokens gets zeros. */
+ * two FP16 parts.  A sequence without tokens gets zeros; of one longer than
+ * its table what the table holds is attended (status 2).  Fewer than 2^31
+ * page reads: batch * kv_heads * (table_stride + sel_stride + 1). */
 int sa_hip_kv4_decode_attention(const sa_paged_kv* kv, const void* query, int32_t type, int64_t q_stride,
                                 const int32_t* selected, const int32_t* counts, int32_t select_groups,
                                 int32_t sel_stride, float scale, void* out, void* workspace,
@@ -791,7 +793,8 @@ int sa_hip_kv4_decode_attention(const sa_paged_kv* kv, const void* query, int32_
  * ascending, at most query_tokens) are the last tokens of sequence b, and
  * the row at position p sees the tokens [0, p].  Rows outside every
  * sequence's range are left as they are.  A sequence with more rows than
- * seq_len (status 4) gets zeros for those before its first token.  Starts
+ * seq_len (status 4) gets zeros for those before its first token; of one
+ * longer than its table what the table holds is attended (status 2).  Starts
  * that do not ascend within [0, query_tokens] attend nothing (status 4). */
 int sa_hip_kv4_prompt_attention(const sa_paged_kv* kv, const void* query, int32_t type, int64_t q_stride,
                                 const int32_t* query_start, int32_t query_tokens, float scale, void* out,

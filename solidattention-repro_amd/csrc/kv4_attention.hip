@@ -593,7 +593,7 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
       tg.n_tokens = t.n_tokens;
       tg.row0 = t.row0;
       limit0 = t.len - t.n_tokens;
-      L = List{nullptr, t.len, 0, 0, (t.len + kPageTokens - 1) / kPageTokens};
+      L = List{nullptr, t.len, 0, 0, pages};
     } else {
       for (;;) {
         b = s / p.select_groups;
@@ -873,6 +873,10 @@ __global__ __launch_bounds__(kTileThreads) void tiles_kernel(const Params p, int
       const int last = min((row0 + rows - 1) / p.group, n - 1);
       const int64_t limit = static_cast<int64_t>(p.seq_len[b]) - n + last;
       pages = limit < 0 ? 1 : static_cast<int>(limit / kPageTokens) + 1;
+      if (pages > p.table_stride) {  // what the table holds of it
+        flag_status(p.status, kStatusBadBlock);
+        pages = p.table_stride;
+      }
     }
     int64_t sum;
     const int64_t pre = scan(pages, sum);

@@ -84,8 +84,13 @@ __device__ inline List decode_list(const Params& p, int b, int sg) {
     if (L.sealed < 0) L.sealed = 0;
     L.len = static_cast<int64_t>(L.sealed) * kPageTokens;
   }
-  const int64_t tail = L.len - static_cast<int64_t>(L.sealed) * kPageTokens;
-  L.total = L.n_sel + static_cast<int>((tail + kPageTokens - 1) / kPageTokens);
+  int64_t tail = (L.len + kPageTokens - 1) / kPageTokens - L.sealed;  // pages
+  const int64_t room = p.table_stride - L.sealed;
+  if (tail > room) {  // what the table holds of it
+    flag_status(p.status, kStatusBadBlock);
+    tail = room > 0 ? room : 0;
+  }
+  L.total = L.n_sel + static_cast<int>(tail);
   return L;
 }
 

@@ -389,7 +389,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_prompt_kernel(const Params p)
     const int b = tile.batch, row0 = tile.row0, pages = tile.pages;
     const int64_t list_first = head * per_head + tile.first;
     const int token0 = tile.token0, n_tokens = tile.n_tokens, len = tile.len;
-    const List L{nullptr, len, 0, 0, (len + kPageTokens - 1) / kPageTokens};
+    const List L{nullptr, len, 0, 0, pages};
     const int p0 = static_cast<int>(u - list_first);
     const int p1 = static_cast<int>(min<int64_t>(pages, p0 + (end - u)));
     const int rows = min(kRows, n_tokens * p.group - row0);          // of the tile

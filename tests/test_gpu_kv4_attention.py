@@ -328,6 +328,58 @@ def test_bad_pages_and_lengths(hip):
     check(out[1, :2], want, K.error_bound(q[1, :2].double().numpy(), k, v, 0.1, "fp32", EPS["fp32"]))
 
 
+def test_lengths_past_the_table(hip):
+    """A length that no table row holds is flagged; its pages end with the row, and the others are as they were."""
+    for lengths, new, dtype in (([60, 100, 33], [1, 1, 1], "fp32"), ([60, 100, 33], [3, 4, 2], "bf16"),
+                                ([60, 100, 33], [60, 100, 33], "bf16")):
+        c = Cache(hip, lengths, 2, 128, 4)
+        c.kv.seq_len[1] = 2 ** 31 - 1
+        start = np.concatenate([[0], np.cumsum(new)])
+        q = query(6, int(start[-1]), 8, 128, dtype)
+        status = ints([0])
+        if max(new) == 1:
+            out = hip.kv4_decode_attention(c.kv, q.cuda(), 0.1, status=status)
+        else:
+            out = hip.kv4_prompt_attention(c.kv, q.cuda(), ints(start), 0.1, status=status)
+        assert int(status) == 2
+        for b in (0, 2):
+            rows = slice(start[b], start[b + 1])
+            c.lengths = [lengths[b]]
+            c.table = c.kv.block_table[b:b + 1].cpu().numpy()
+            check_prompt(c, q[rows], [0, new[b]], out[rows], dtype, 0.1)
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "fp16"), (128, "fp16"), (64, "bf16"), (128, "bf16")])
+def test_nan_in_tiles_of_many_rows(hip, d, dtype):
+    """A NaN value reaches the channels of its group, a NaN key its head, in the rows that see the token."""
+    lengths = [400, 70]
+    c = Cache(hip, lengths, 2, d, 4)
+    g = torch.Generator().manual_seed(3)
+    k, v = torch.randn((1, 2, d), generator=g), torch.randn((1, 2, d), generator=g)
+    v[0, 0, 40] = float("nan")       # head 0, channels 32..63 of token 80
+    hip.kv4_store(c.kv, k.cuda(), v.cuda(), ints([c.table[0, 2] * 32 + 16]))
+    k[0, 1, 3], v[0, 0, 40] = float("nan"), 0.5
+    hip.kv4_store(c.kv, k.cuda(), v.cuda(), ints([c.table[0, 6] * 32 + 31]))  # head 1's key of token 223
+    c.refresh()
+    q = query(3, 470, 8, d, dtype)
+    out = hip.kv4_prompt_attention(c.kv, q.cuda(), ints([0, 400, 470]), 0.09).cpu()
+    nan = torch.zeros(out.shape, dtype=torch.bool)
+    nan[80:400, :4, 32:64] = True
+    nan[223:400, 4:] = True
+    assert torch.equal(out.isnan(), nan)
+    for b, at in ((0, 0), (1, 400)):
+        for h in range(2):
+            k, v = c.rows(b, h, np.arange((lengths[b] + 31) // 32), lengths[b])
+            k, v = np.nan_to_num(k), np.nan_to_num(v)
+            for i in range(0, lengths[b], 13):
+                rows = slice(4 * h, 4 * h + 4)
+                qq, on = q[at + i, rows].double().numpy(), out[at + i, rows].double().numpy()
+                want, _ = K.attend(qq, k[:i + 1], v[:i + 1], 0.09)
+                bound = K.error_bound(qq, k[:i + 1], v[:i + 1], 0.09, dtype, EPS[dtype], rounded=True)
+                keep = ~nan[at + i, rows].numpy()
+                assert (np.abs(on - want)[keep] <= np.broadcast_to(bound, on.shape)[keep]).all(), (b, h, i)
+
+
 def test_strided_query_own_buffer_and_stream(hip):
     """Rows inside a fused projection; out over the query; a stream other than the current one."""
     c = Cache(hip, [90, 300, 64], 2, 128, 4)

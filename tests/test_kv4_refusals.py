@@ -95,6 +95,8 @@ def test_attention_arguments():
     refused(decode(sel=P, cnt=P, g=0, ss=4), "select_groups")
     refused(decode(sel=P, cnt=P, g=3, ss=4), "select_groups")
     refused(decode(sel=P, cnt=P, g=2, ss=0), "sel_stride")
+    refused(L.sa_hip_kv4_decode_attention(C.byref(struct(batch=64, table_stride=1 << 25)), P, 1, 512, None, None, 0, 0,
+                                          one, O, P, 1 << 40, None, None), "2^31 page reads")
     refused(decode(out=C.c_void_p((1 << 20) + 512)), "overlap")
     prompt = lambda st=P, n=5, q=P, qs=512, out=O, ws=1 << 40: \
         L.sa_hip_kv4_prompt_attention(kv, q, 1, qs, st, n, one, out, P, ws, None, None)
