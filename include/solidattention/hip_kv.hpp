@@ -26,6 +26,8 @@
 //                              misses are copied, then of the misses, merged
 //                              (the overlap of pipeline_main.cpp:811-848)
 //   compare_prediction         pipeline_main.cpp:686-717
+// PageStack and PagedKv4Pool (pages handed out on the GPU, pages held in 4
+// bits and the attention over them) have no counterpart in the reference.
 // Errors are std::runtime_error("operation: message"), as the reference's
 // cuda_check does (cuda_backend.cpp:16-21).
 #pragma once
@@ -167,6 +169,132 @@ class PagedKvPool {
   DeviceArray<std::uint16_t> pool_;
   DeviceArray<int32_t> table_, seq_len_, sealed_, generation_;
   DeviceArray<float> reps_;
+};
+
+// The free pages of a pool as a stack on the device, and the places that the
+// last reserve() gave out: query_start [batch + 1], slots and positions
+// [max_tokens].  Works on either pool's view.
+class PageStack {
+ public:
+  // Every page of the pool is free, the last ids on top.
+  PageStack(std::size_t num_pages, std::size_t batch, std::size_t max_tokens)
+      : free_(num_pages), count_(1), start_(batch + 1), slots_(max_tokens), positions_(max_tokens) {
+    std::vector<int32_t> ids(num_pages);
+    for (std::size_t i = 0; i < num_pages; ++i) ids[i] = static_cast<int32_t>(i);
+    free_.upload(ids);
+    count_.upload({static_cast<int32_t>(num_pages)});
+  }
+  // Pages and slots for new_tokens[b] (device) more tokens of each sequence.
+  // seq_len is advanced unless next_len (device) takes the new lengths.
+  void reserve(const sa_paged_kv& kv, const int32_t* new_tokens, int32_t* next_len = nullptr,
+               hipStream_t stream = nullptr, int32_t* status = nullptr) {
+    check(sa_hip_reserve_tokens(&kv, new_tokens, free_.get(), count_.get(), static_cast<int32_t>(slots_.size()),
+                                start_.get(), slots_.get(), positions_.get(),
+                                next_len ? next_len : const_cast<int32_t*>(kv.seq_len), count_.get(), status, stream),
+          "reserve_tokens");
+  }
+  // The pages of the sequences with finished[b] != 0 (device) go back.
+  void release(const sa_paged_kv& kv, const int32_t* finished, hipStream_t stream = nullptr,
+               int32_t* status = nullptr) {
+    check(sa_hip_release_sequences(&kv, finished, free_.get(), count_.get(), const_cast<int32_t*>(kv.seq_len),
+                                   count_.get(), status, stream),
+          "release_sequences");
+  }
+  DeviceArray<int32_t>& free_pages() { return free_; }
+  DeviceArray<int32_t>& count() { return count_; }
+  DeviceArray<int32_t>& query_start() { return start_; }
+  DeviceArray<int32_t>& slots() { return slots_; }
+  DeviceArray<int32_t>& positions() { return positions_; }
+
+ private:
+  DeviceArray<int32_t> free_, count_, start_, slots_, positions_;
+};
+
+// One layer's cache with its pages held in 4 bits (head_dim 64, 128 or 256),
+// and the attention workspace for up to max_tokens query rows a call.  Tokens,
+// queries and outputs are of `type` (SA_HIP_F32, SA_HIP_F16 or SA_HIP_BF16),
+// [tokens][heads][head_dim], contiguous.
+class PagedKv4Pool {
+ public:
+  PagedKv4Pool(std::size_t batch, std::size_t query_heads, std::size_t kv_heads, std::size_t table_stride,
+               std::size_t num_pages, std::size_t head_dim = 128, std::size_t max_tokens = 0)
+      : tables_(batch, query_heads, kv_heads, table_stride, 0, 0, 0, head_dim), num_pages_(num_pages),
+        page_bytes_(bytes_of(kv_heads, head_dim)), pool_(num_pages * page_bytes_),
+        workspace_bytes_(workspace_of(max_tokens ? max_tokens : batch)), workspace_((workspace_bytes_ + 3) / 4) {}
+
+  std::size_t page_bytes() const { return page_bytes_; }
+  sa_paged_kv view() const {
+    sa_paged_kv v = tables_.view();
+    v.pool = reinterpret_cast<decltype(v.pool)>(pool_.get());
+    v.num_pages = static_cast<int64_t>(num_pages_);
+    v.reserved = SA_HIP_POOL_KV4;
+    return v;
+  }
+  DeviceArray<std::uint8_t>& pool() { return pool_; }
+  DeviceArray<int32_t>& block_table() { return tables_.block_table(); }
+  DeviceArray<int32_t>& seq_len() { return tables_.seq_len(); }
+  DeviceArray<int32_t>& sealed() { return tables_.sealed(); }
+  DeviceArray<int32_t>& generation() { return tables_.generation(); }
+  DeviceArray<float>& reps() { return tables_.reps(); }
+
+  void store(const void* k, const void* v, int type, const int32_t* slots, int tokens, hipStream_t stream = nullptr,
+             int32_t* status = nullptr) {
+    const sa_paged_kv kv = view();
+    check(sa_hip_kv4_store(&kv, k, v, type, row(kv.kv_heads), row(kv.kv_heads), slots, tokens, status, stream),
+          "kv4_store");
+  }
+  void load(void* k, void* v, int type, const int32_t* slots, int tokens, hipStream_t stream = nullptr,
+            int32_t* status = nullptr) {
+    const sa_paged_kv kv = view();
+    check(sa_hip_kv4_load(&kv, k, v, type, row(kv.kv_heads), row(kv.kv_heads), slots, tokens, status, stream),
+          "kv4_load");
+  }
+  void append_seal(const void* k, const void* v, int type, int local_tokens, hipStream_t stream = nullptr,
+                   int32_t* status = nullptr) {
+    const sa_paged_kv kv = view();
+    check(sa_hip_kv4_append_seal(&kv, k, v, type, row(kv.kv_heads), row(kv.kv_heads), local_tokens, status, stream),
+          "kv4_append_seal");
+  }
+  void seal(int local_tokens, hipStream_t stream = nullptr, int32_t* status = nullptr) {
+    const sa_paged_kv kv = view();
+    check(sa_hip_kv4_seal(&kv, local_tokens, status, stream), "kv4_seal");
+  }
+  // One token a sequence over the selected blocks and the tail (selected and
+  // counts as sa_hip_score_select gives them), or over every token.
+  void decode(const void* query, int type, float scale, void* out, const int32_t* selected = nullptr,
+              const int32_t* counts = nullptr, int select_groups = 0, int sel_stride = 0,
+              hipStream_t stream = nullptr, int32_t* status = nullptr) {
+    const sa_paged_kv kv = view();
+    check(sa_hip_kv4_decode_attention(&kv, query, type, row(kv.query_heads), selected, counts, select_groups,
+                                      sel_stride, scale, out, workspace_.get(), workspace_bytes_, status, stream),
+          "kv4_decode_attention");
+  }
+  // Rows [query_start[b], query_start[b + 1]) are the last tokens of sequence b.
+  void prompt(const void* query, int type, const int32_t* query_start, int tokens, float scale, void* out,
+              hipStream_t stream = nullptr, int32_t* status = nullptr) {
+    const sa_paged_kv kv = view();
+    check(sa_hip_kv4_prompt_attention(&kv, query, type, row(kv.query_heads), query_start, tokens, scale, out,
+                                      workspace_.get(), workspace_bytes_, status, stream),
+          "kv4_prompt_attention");
+  }
+
+ private:
+  static std::size_t bytes_of(std::size_t kv_heads, std::size_t head_dim) {
+    const std::size_t n = sa_hip_kv4_page_bytes(static_cast<int32_t>(kv_heads), static_cast<int32_t>(head_dim));
+    if (!n) throw std::runtime_error("PagedKv4Pool: 4-bit pages have head_dim 64, 128 or 256");
+    return n;
+  }
+  std::size_t workspace_of(std::size_t tokens) const {
+    const sa_paged_kv kv = view();
+    return sa_hip_kv4_attention_workspace_bytes(&kv, static_cast<int32_t>(tokens));
+  }
+  int64_t row(int32_t heads) const { return static_cast<int64_t>(heads) * static_cast<int64_t>(tables_.head_dim()); }
+
+  PagedKvPool tables_;  // without pages of its own
+  std::size_t num_pages_, page_bytes_;
+  DeviceArray<std::uint8_t> pool_;
+  std::size_t workspace_bytes_;
+  DeviceArray<int32_t> workspace_;  // zero-filled, as the calls leave it
 };
 
 // Budgeted selection + sparse decode attention with the scratch they need.

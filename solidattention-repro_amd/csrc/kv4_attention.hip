@@ -24,6 +24,15 @@
 // lists form one row of units, and each workgroup takes an equal share of it,
 // whatever the lists' lengths.  A list cut by a share's border is merged by the
 // last workgroup to finish it.
+//
+// What bounds it: memory, where the batch is long (8 sequences of up to 131072
+// tokens in groups of 4: 184-193 us, 5.2-5.4 TB/s); below that the vector
+// instructions of a page (225 at head_dim 64, 325 at 128, 570 for 32 rows, 4
+// cycles each: 32 sequences of 5000 to 10000 tokens at head_dim 64 42.7 us, 3.6
+// TB/s; 64 of 64 selected blocks in fp32 47 us, 3.6 TB/s); for one sequence of
+// 2048 tokens, 11.4 us, the chain length -> table -> record -> sums -> counter
+// -> sums of a launch.  The code outside the loop counts there too: fetching it
+// for the first time takes longer than running it.
 #include "kv4_attention.hpp"
 
 #include <algorithm>
@@ -507,7 +516,7 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
   unit_t base = 0;  // units before list (decode: the lists of one selection group's heads) or tile s
   int s = 0;
   if constexpr (kCausal) {
-    const Start at = start_share(p, sh, w, kMinUnits, lane);
+    const Start at = start_share(p, sh, w, kWholePagesOfMany, lane);
     if (!at.any) return;
     s = at.s;
     u = at.u;
@@ -531,46 +540,47 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
     const uint32_t run = wave_prefix_sum(mine);
     const uint32_t head = __builtin_amdgcn_readfirstlane(one);
     even = __all(even && (first == last || one == head));
-    const bool brief = __all(most <= kWholePages);
+    const uint32_t all = static_cast<uint32_t>(lists) * p.kv_per_sel;
+    const bool whole = __all(whole_lists(all, most, kWholePagesOfMany));
     if (lane == kWave - 1) {
       s_units[wave] = run;
       s_first[wave] = head;
-      s_even[wave] = even | brief << 1;
+      s_even[wave] = even | whole << 1;
     }
     __syncthreads();
     uint32_t before = 0;
-    bool alike = true, all_brief = true;
+    bool alike = true, all_whole = true;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
       if (i < wave) before += s_units[i];
       sh.units += s_units[i];
-      all_brief = all_brief && s_even[i] & 2;
-      alike = alike && s_even[i] & 1 && (s_first[i] == s_first[0] || s_units[i] == 0);
+      all_whole = all_whole && (s_even[i] & 2) != 0;
+      alike = alike && (s_even[i] & 1) != 0 && (s_first[i] == s_first[0] || s_units[i] == 0);
     }
     sh.groups = min(gridDim.x, max(1u, sh.units / kMinUnits));
-    // Lists of one length are cut into as many shares each, so that no share
-    // crosses from one into the next: one that does writes its sums twice.
-    const uint32_t all = static_cast<uint32_t>(lists) * p.kv_per_sel;
-    if (all_brief && all <= gridDim.x) {
+    if (all_whole) {
       if (w >= all) return;
       s = w / p.kv_per_sel;
       const uint32_t pages = max(decode_list(p, s / p.select_groups, s % p.select_groups).total, 1);
       u = w % p.kv_per_sel * pages;  // of the list's own units
       end = u + pages;
     } else {
-    if (alike && all <= gridDim.x) sh.groups = all * max(1u, sh.groups / all);
-    if (w >= sh.groups) return;
-    sh.divide();
-    u = sh.begin(w);
-    end = sh.begin(w + 1);
-    before += run - mine;
-    if (u - before < mine) {  // (u < before wraps to more than any)
-      s_found[0] = first;
-      s_found[1] = before;
-    }
-    __syncthreads();
-    s = __builtin_amdgcn_readfirstlane(s_found[0]);
-    base = __builtin_amdgcn_readfirstlane(s_found[1]);
+      // Lists of one length are cut into as many shares each, so that no share
+      // crosses from one into the next: one that does writes its sums twice
+      // (512 lists of 64 blocks: 57 -> 45 us).
+      if (alike && all <= gridDim.x) sh.groups = all * max(1u, sh.groups / all);
+      if (w >= sh.groups) return;
+      sh.divide();
+      u = sh.begin(w);
+      end = sh.begin(w + 1);
+      before += run - mine;
+      if (u - before < mine) {  // (u < before wraps to more than any)
+        s_found[0] = first;
+        s_found[1] = before;
+      }
+      __syncthreads();
+      s = __builtin_amdgcn_readfirstlane(s_found[0]);
+      base = __builtin_amdgcn_readfirstlane(s_found[1]);
     }
   }
 
@@ -593,7 +603,7 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, RT>)) void kv4_attention_kerne
       tg.n_tokens = t.n_tokens;
       tg.row0 = t.row0;
       limit0 = t.len - t.n_tokens;
-      L = List{nullptr, t.len, 0, 0, pages};
+      L = List{nullptr, t.len, 0, 0, static_cast<int>((static_cast<uint32_t>(t.len) + kPageTokens - 1) / kPageTokens)};
     } else {
       for (;;) {
         b = s / p.select_groups;
@@ -909,7 +919,10 @@ int grid_groups(int head_dim, int RT) {
 
 // How a call runs: one token a sequence in a tile of 16 rows; several in this
 // file's tiles of 32 rows (16 at head_dim 256, by the registers), or in
-// kv4_prompt.hip's of many.
+// kv4_prompt.hip's of many, from 96 rows a sequence (per KV head) on: 16
+// sequences after 8192 tokens, 8 heads of 128, take 86 us in few and 129 in
+// many at 48 rows, 150 and 143 at 96, 250 and 161 at 192; after 1024 tokens 27
+// and 39, 36 and 43, 50 and 44.
 enum class Form { kDecode, kFew, kMany };
 
 struct Plan {
@@ -926,7 +939,7 @@ Plan plan(Form form, int head_dim) {
 
 Form form_of(bool prompt, int64_t tokens, int64_t batch, int group, int head_dim, int type) {
   if (!prompt) return Form::kDecode;
-  return type != kF32 && head_dim <= 128 && tokens * group >= 64 * batch ? Form::kMany : Form::kFew;
+  return type != kF32 && head_dim <= 128 && tokens * group >= 96 * batch ? Form::kMany : Form::kFew;
 }
 
 struct Layout {

@@ -214,9 +214,18 @@ struct Share {
   __device__ inline int64_t owner(int64_t u) const { return ((u + 1) * groups - 1) / units; }
 };
 
-// Lists of at most this many pages, a workgroup for each, are not cut: the
-// shares' sums would take longer to meet than the pages to be attended.
+// Lists of few pages, a workgroup for each, are not cut: the shares' sums would
+// take longer to meet than the pages to be attended.  With lists for a quarter
+// of the launch's workgroups, which then share the memory's rate, that holds
+// for longer ones (256 lists at head_dim 64, cut and whole: up to 2 pages 30
+// and 7.5 us, 16 pages 17.2 and 10.0, 32 pages 17.3 and 12.9, 63 pages 21.2 and
+// 18.4); not for tiles of many rows, whose pages take ten times as long.
 constexpr int kWholePages = 16;
+constexpr int kWholePagesOfMany = 48;
+__device__ inline bool whole_lists(int64_t lists, int64_t longest, int many) {
+  return lists <= static_cast<int64_t>(gridDim.x) &&
+         longest <= (lists * 4 >= static_cast<int64_t>(gridDim.x) ? many : kWholePages);
+}
 
 // `rows` rows (token * group + head) of one sequence, for every KV head.
 struct Tile {
@@ -250,17 +259,17 @@ struct Start {
   int64_t u, end;
   bool any;
 };
-__device__ inline Start start_share(const Params& p, Share& sh, int64_t w, int min_units, int lane) {
+__device__ inline Start start_share(const Params& p, Share& sh, int64_t w, int whole_of_many, int lane) {
   const int64_t tiles = p.tile_info[0], per_head = p.tile_info[1], longest = p.tile_info[2];
   sh.units = per_head * p.kv_heads;
   if (sh.units <= 0) return Start{0, 0, 0, false};
-  if (tiles * p.kv_heads <= static_cast<int64_t>(gridDim.x) && longest <= kWholePages) {
+  if (whole_lists(tiles * p.kv_heads, longest, whole_of_many)) {
     if (w >= tiles * p.kv_heads) return Start{0, 0, 0, false};
     const int s = static_cast<int>(w) % static_cast<int>(tiles);
     const int64_t u = static_cast<int>(w) / static_cast<int>(tiles) * per_head + p.tiles[s].first;
     return Start{s, u, u + p.tiles[s].pages, true};
   }
-  sh.groups = min<int64_t>(gridDim.x, max<int64_t>(1, sh.units / min_units));
+  sh.groups = min<int64_t>(gridDim.x, max<int64_t>(1, sh.units / kMinUnits));
   if (w >= sh.groups) return Start{0, 0, 0, false};
   const int64_t u = sh.begin(w);
   return Start{find_tile(p, u % per_head, lane), u, sh.begin(w + 1), true};

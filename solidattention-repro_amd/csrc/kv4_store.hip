@@ -1,11 +1,16 @@
 // kv4_store.hip — writes tokens into the 4-bit pages, reads them back, and
 // keeps the block representatives of such a cache (gfx950).
 //
-// All of it is bound by memory.  A lane handles 8 channels of one row, so a
-// group of 32 channels is a quad of lanes whose minimum and maximum meet by
-// DPP; a wave covers 512 / D tokens of one head, adjacent waves adjacent
-// heads, so the reads of k and v are whole rows and the codes of 4 adjacent
-// tokens fill the record's lines together.
+// A lane handles 8 channels of one row, so a group of 32 channels is a quad of
+// lanes whose minimum and maximum meet by DPP; a wave covers 512 / D tokens of
+// one head, adjacent waves adjacent heads, so the reads of k and v are whole
+// rows and the codes of 4 adjacent tokens fill the record's lines together.
+// 16384 tokens, 8 heads of 128, BF16: the store takes 27 us (3.3 TB/s, bound by
+// the 400 vector instructions of a wave's 8 values of k and of v), the load 18.5
+// (4.8 TB/s, bound by memory).  A workgroup for all of a page, so that no line
+// is written from two dies, made the store slower (36 against 33 us).
+// Append + seal of one token for 64 sequences: 7.1 us, the chain length ->
+// table -> record -> mean.
 #include "kv4_format.hpp"
 #include "sa_internal.hpp"
 

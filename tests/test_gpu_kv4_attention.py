@@ -100,10 +100,11 @@ def test_decode_batches(hip, B):
 
 
 @pytest.mark.parametrize("d,lengths", [(64, [1, 512, 0, 40]), (128, [300] * 5), (128, [512, 511]), (256, [33, 64, 2]),
-                                       (128, [513, 20]), (64, [2000] * 3), (128, [700] * 40)])
+                                       (128, [513, 20]), (64, [2000] * 3), (128, [700] * 40),
+                                       (64, [1536, 3, 900, 1100] * 13), (128, [1537, 40] * 26)])
 def test_decode_short_and_equal_lists(hip, d, lengths):
-    """Lists of up to 16 pages with a workgroup each, one page more, and lists of one length, whose shares end with
-    them; whole sequences and selected blocks."""
+    """Lists of up to 16 pages with a workgroup each, of up to 48 when there are many, one page more, and lists of one
+    length, whose shares end with them; whole sequences and selected blocks."""
     c = Cache(hip, lengths, 4, d, 2, seed=7)
     q = query(8, len(lengths), 8, d, "fp32")
     status = ints([0])
@@ -121,7 +122,8 @@ def test_decode_short_and_equal_lists(hip, d, lengths):
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_prompt_short_lists(hip, d, dtype):
     """Tiles of up to 16 pages with a workgroup each, in tiles of few rows and of many, and tiles of one page more."""
-    for lengths, new in (([512, 40, 3], [4, 2, 3]), ([512, 100], [512, 100]), ([513, 100], [3, 4]), ([530], [400])):
+    for lengths, new in (([512, 40, 3], [4, 2, 3]), ([512, 100], [512, 100]), ([513, 100], [3, 4]), ([530], [400]),
+                         ([1536, 900] * 33, [3, 2] * 33), ([1537, 8] * 33, [2, 3] * 33)):
         c = Cache(hip, lengths, 2, d, 4, seed=6)
         start = np.concatenate([[0], np.cumsum(new)])
         q = query(9, int(start[-1]), 8, d, dtype)
