@@ -27,7 +27,7 @@
 // its part of the page's conversion).  Two waves a SIMD run them against each
 // other.  32 rows a wave keep its LDS reads (16 KB a page) under the matrix
 // cores' time.  Measured, head_dim 128: 8 chunks of up to 1024 tokens after up
-// to 15360, groups of 4, FP16, 1610 us, 780 TFLOP/s; one prompt of 4096 tokens,
+// to 15360, groups of 4, FP16, 1610-1650 us, 770 TFLOP/s; one prompt of 4096 tokens,
 // BF16, 163 us, 420 TFLOP/s, of which 40 us are the meeting of cut tiles' sums
 // and as much the start of each tile.  (The conversion costs a quarter of the
 // time; both pages of a pair from one record: 3% less.)
