@@ -382,6 +382,38 @@ def test_nan_in_tiles_of_many_rows(hip, d, dtype):
                 assert (np.abs(on - want)[keep] <= np.broadcast_to(bound, on.shape)[keep]).all(), (b, h, i)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_nan_in_tiles_of_few_rows(hip, d, dtype):
+    """The same among the last tokens of a sequence, whose rows see a part of their page."""
+    c = Cache(hip, [400, 70], 2, d, 4)
+    g = torch.Generator().manual_seed(3)
+    k, v = torch.randn((1, 2, d), generator=g), torch.randn((1, 2, d), generator=g)
+    v[0, 0, 40] = float("nan")       # head 0, channels 32..63 of token 395
+    hip.kv4_store(c.kv, k.cuda(), v.cuda(), ints([c.table[0, 12] * 32 + 11]))
+    k[0, 1, 3], v[0, 0, 40] = float("nan"), 0.5
+    hip.kv4_store(c.kv, k.cuda(), v.cuda(), ints([c.table[0, 12] * 32 + 13]))  # head 1's key of token 397
+    c.refresh()
+    q = query(3, 14, 8, d, dtype)
+    out = hip.kv4_prompt_attention(c.kv, q.cuda(), ints([0, 9, 14]), 0.09).cpu()  # tokens 391.., 65..
+    nan = torch.zeros(out.shape, dtype=torch.bool)
+    nan[4:9, :4, 32:64] = True
+    nan[6:9, 4:] = True
+    assert torch.equal(out.isnan(), nan)
+    for b, at, m in ((0, 0, 9), (1, 9, 5)):
+        n = c.lengths[b]
+        for h in range(2):
+            k, v = c.rows(b, h, np.arange((n + 31) // 32), n)
+            k, v = np.nan_to_num(k), np.nan_to_num(v)
+            for i in range(m):
+                rows, seen = slice(4 * h, 4 * h + 4), n - m + i + 1
+                qq, on = q[at + i, rows].double().numpy(), out[at + i, rows].double().numpy()
+                want, _ = K.attend(qq, k[:seen], v[:seen], 0.09)
+                bound = K.error_bound(qq, k[:seen], v[:seen], 0.09, dtype, EPS[dtype])
+                keep = ~nan[at + i, rows].numpy()
+                assert (np.abs(on - want)[keep] <= np.broadcast_to(bound, on.shape)[keep]).all(), (b, h, i)
+
+
 def test_strided_query_own_buffer_and_stream(hip):
     """Rows inside a fused projection; out over the query; a stream other than the current one."""
     c = Cache(hip, [90, 300, 64], 2, 128, 4)
