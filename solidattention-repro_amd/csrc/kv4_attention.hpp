@@ -188,7 +188,9 @@ __device__ inline float ldexp2(float x, int e) { return __builtin_ldexpf(x, e); 
 // The pages of all lists form one row of units; workgroup w of `groups` takes
 // units [begin(w), begin(w + 1)), whatever lists they belong to.
 
-struct SmallShare {  // fewer than 2^31 units, at most 4096 groups
+// One token a sequence: fewer than 2^31 units (refused otherwise), at most 4096
+// groups.
+struct SmallShare {
   uint32_t units;    // of the whole launch
   uint32_t groups;   // workgroups that take part
   uint32_t each, rest;  // units = each * groups + rest
@@ -207,6 +209,8 @@ struct SmallShare {  // fewer than 2^31 units, at most 4096 groups
   }
 };
 
+// Tiles of many tokens may pass 2^31 units.  (The 32-bit form for fewer cost
+// more than it saved there: 42 against 36 us for 16 sequences of 5 tokens.)
 struct Share {
   int64_t units;
   int64_t groups;
